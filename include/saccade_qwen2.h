@@ -12,6 +12,12 @@
  *                             heuristics.rs:3-14) in their epilogue, consumed by
  *                             sc_forward_group_routed
  *   sc_qwen2_f16_to_f32    <- ProjectionLayer::forward's to_dtype back to f32  model.rs:61
+ *   sc_qwen2_paged_append, sc_qwen2_paged_attention
+ *                          <- the two cache steps on a paged cache of f32, f16 or bf16 shared by ragged
+ *                             sequences (the reference concatenates one f32 tensor per sequence)
+ *   sc_qwen2_process_logits
+ *                          <- penalties, biases and grammar masks before the argmax of
+ *                             saccade-runner/src/bin/verify.rs:98-130 (the reference has the argmax only)
  *
  * The linears themselves are sc_forward / sc_forward_group calls (saccade_ctarq.h).  Everything is
  * f32 except the inputs of the linears, which these kernels write as f16 (the projection layer's
@@ -90,6 +96,81 @@ SC_API sc_status sc_qwen2_silu_mul_route(const uint16_t* gate, const uint16_t* u
                                          uint16_t* out_f16, const sc_group* group, uint8_t* const* mask,
                                          int32_t* const* routed_idx, int32_t* const* n_routed, uint32_t* counter,
                                          void* stream);
+
+/* ---- A paged cache.  k_pages / v_pages hold num_pages pages of [num_kv_heads][page_size][head_dim]
+ * elements of cache_dtype (SC_F32, SC_F16, SC_BF16), page p at element p * page_stride (each page's
+ * own elements contiguous).  Row b of block_table [num_seqs][max_pages] lists sequence b's pages in
+ * order: its position p is row p % page_size of page block_table[b][p / page_size].  Sequence b owns
+ * token rows cu_q[b] .. cu_q[b + 1] (cu_q [num_seqs + 1], ascending from 0; rows from cu_q[num_seqs] on
+ * belong to no sequence and their outputs are left as they were) and kv_len[b] positions counting those
+ * tokens: its i-th new token sits at position kv_len[b] - (cu_q[b + 1] - cu_q[b]) + i.  All of these are
+ * device arrays read by the kernels, so a captured graph replays with new lengths and pages.
+ * Limits (SC_EINVAL otherwise): head_dim 64 or 128; page_size a power of two in 8..256; num_heads a
+ * multiple of num_kv_heads with at most 64 query heads per KV head.  Nothing of a page is read or
+ * written that the lengths do not cover, except that attention may load the rest of a sequence's
+ * last page, whatever it holds.  A position, page or length outside the tables records SC_EDEVICE in
+ * *status (nullable device word; see sc_layer_check's codes) and is skipped, never followed. */
+
+/* Rotates q and k (out[d] = x[d] cos[d] - x[d + hd/2] sin[d], out[d + hd/2] = x[d + hd/2] cos[d + hd/2] +
+ * x[d] sin[d + hd/2] in f32, with row `position` of cos_table / sin_table [max_pos][head_dim]), writes
+ * the rotated k and v into the pages and the rotated q to q_out [tokens][num_heads][head_dim], all as
+ * cache_dtype with one rounding.  q, k, v: in_dtype rows (heads contiguous) q_stride, k_stride and
+ * v_stride elements apart, so slices of one projection buffer serve.  in_dtype is SC_F32 or
+ * cache_dtype.  q_out may be q itself (same type, q_stride = num_heads * head_dim).  A token whose
+ * position lies outside the rotation tables is left out; one without a page gets its q only. */
+SC_API sc_status sc_qwen2_paged_append(const void* q, const void* k, const void* v, int in_dtype, int64_t q_stride,
+                                       int64_t k_stride, int64_t v_stride, int64_t tokens, const float* cos_table,
+                                       const float* sin_table, int64_t max_pos, int num_heads, int num_kv_heads,
+                                       int head_dim, void* k_pages, void* v_pages, int cache_dtype, int64_t num_pages,
+                                       int64_t page_stride, int page_size, const int32_t* block_table,
+                                       int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len, int64_t num_seqs,
+                                       void* q_out, uint32_t* status, void* stream);
+
+/* Scratch bytes sc_qwen2_paged_attention needs (no initial contents; one call uses it at a time). */
+SC_API size_t sc_qwen2_paged_attention_scratch(int64_t tokens, int64_t num_seqs, int num_heads, int num_kv_heads,
+                                               int head_dim, int64_t max_q_len, int cache_dtype);
+
+/* Causal attention of each sequence's new tokens over its pages: the token at position p attends
+ * positions 0..p, o = sum softmax(scale * q . k) v per query head (grouped onto the KV heads), f32
+ * sums and softmax statistics.  q [tokens][num_heads][head_dim] of cache_dtype, rows q_stride elements
+ * apart; out [tokens][num_heads][head_dim] contiguous, out_dtype = cache_dtype (an f32 cache may also
+ * write SC_F16, the linears' input).  lse (nullable, f32 [tokens][num_heads]) = log sum exp(scale * q . k).
+ * A token at a negative position attends nothing: its output is 0, its lse -inf.  max_q_len bounds
+ * every sequence's new tokens (one sequence beyond it is skipped and recorded); max_kv_len is the
+ * cached positions' bound.  16-bit caches need q, the pages and their strides 16-byte aligned and run
+ * on the tensor cores; cached values at covered positions must be finite. */
+SC_API sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                                          int cache_dtype, int64_t num_pages, int64_t page_stride, int page_size,
+                                          const int32_t* block_table, int64_t max_pages, const int32_t* cu_q,
+                                          const int32_t* kv_len, int64_t num_seqs, int64_t tokens, int num_heads,
+                                          int num_kv_heads, int head_dim, int64_t max_q_len, int64_t max_kv_len,
+                                          float scale, void* out, int out_dtype, float* lse, void* scratch,
+                                          size_t scratch_bytes, uint32_t* status, void* stream);
+
+/* Logits [rows][vocab] of dtype (SC_F32, SC_F16, SC_BF16), rows `stride` apart, of the tokens vocab_begin ..
+ * vocab_begin + vocab (a tensor-parallel rank's slice; every id below is of the whole vocabulary) ->
+ * out (out_stride apart; may be logits itself).  Per row and token v, in f32 and rounded once:
+ *   x = logits[v]
+ *   v among the row's history: x = x > 0 ? x / repetition : x * repetition
+ *   x = x - frequency * n - (n > 0 ? presence : 0), n = times v occurs among the generated tokens
+ *   x = x + the last bias entry of v;   x = -inf where the row's grammar mask does not allow v
+ * history [rows][history_stride] (ids; others than the slice's are passed over): the first hist_len[r]
+ * are the row's, of these the first prompt_len[r] its prompt (null prompt_len: all generated).
+ * repetition, presence, frequency: f32 per row (null: 1, 0, 0).  bias entries bias_ptr[r] .. bias_ptr[r + 1]
+ * of bias_ids / bias_vals [num_bias], at most 4095 a row.  mask [mask_rows][mask_words] of bits, bit v % 32
+ * of word v / 32: 1 allows v; mask_row[r] is the row's mask, negative for none (null mask_row: mask r).
+ * best (nullable int64 [rows]) and best_value (nullable, dtype [rows]): the id and value of the largest
+ * output, the first of equals, NaN above all as torch.argmax has it.  A length, mask row or number of
+ * bias entries out of range records SC_EDEVICE in *status (nullable) and is cut to what there is (a
+ * mask row: no mask).  history_stride <= 524287 and vocab <= 2^30, SC_EINVAL otherwise. */
+SC_API sc_status sc_qwen2_process_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
+                                         int64_t vocab_begin, const int32_t* history, int64_t history_stride,
+                                         const int32_t* prompt_len, const int32_t* hist_len, const float* repetition,
+                                         const float* presence, const float* frequency, const int32_t* bias_ptr,
+                                         const int32_t* bias_ids, const float* bias_vals, int64_t num_bias,
+                                         const int32_t* mask, int64_t mask_words, int64_t mask_rows,
+                                         const int32_t* mask_row, void* out, int64_t out_stride, int64_t* best,
+                                         void* best_value, uint32_t* status, void* stream);
 
 SC_API sc_status sc_qwen2_f16_to_f32(const uint16_t* x, int64_t n, float* out, void* stream);
 

@@ -1,0 +1,369 @@
+// sc_paged.cu -- the paged KV cache: rotation and appending of new tokens, and causal attention of the
+// new tokens over the pages.
+#include <atomic>
+#include <string>
+
+#include "saccade_qwen2.h"
+#include "sc_device.cuh"
+#include "sc_internal.h"
+#include "sc_paged.cuh"
+
+namespace sc {
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// ---------------------------------------------------------------- rotation + append
+// A thread has 8 rotated pairs (elements d..d+7 and d+hd/2..d+hd/2+7) of one token and takes the
+// heads in turn, so that the token's angles are loaded once for all of its heads; q, k and v heads
+// follow one another in the loop.  Bytes bound: q, k, v read, q' and the cache rows written, two
+// table rows per token.
+constexpr int kAppendThreads = 256;
+
+struct AppendArgs {
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride;
+    const float *cos_t, *sin_t;
+    int64_t max_pos;
+    void *kp, *vp, *q_out;
+    PagedKv c;
+    int vec_in;      // q, k, v rows start on 16-byte boundaries
+    int vec_cache;   // the pages do
+    int vec_table;   // the rotation tables do
+    int vec_qout;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, float (&f)[8]) {
+    if (vec) {
+        __align__(16) T t[8];
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+            reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(p[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool vec, const float (&f)[8]) {
+    __align__(16) T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(f[i]);
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+            reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = t[i];
+    }
+}
+
+template <typename In, typename Cache, int kHd>
+__global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArgs a) {
+    constexpr int kHalf = kHd / 2;
+    constexpr int kChunks = kHalf / 8;                 // threads of one head
+    constexpr int kHeads = kAppendThreads / kChunks;   // heads taken at a time
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 31;
+    // the token's sequence: the number of sequences that end at or before it
+    int seq = 0;
+    for (int b0 = 0; b0 < a.c.num_seqs; b0 += 32) {
+        const bool before = b0 + lane < a.c.num_seqs && a.c.cu_q[b0 + lane + 1] <= t;
+        seq += __popc(__ballot_sync(0xffffffffu, before));
+    }
+    if (seq >= a.c.num_seqs || t < a.c.cu_q[seq]) return;  // a row behind the last sequence
+    const int64_t pos = static_cast<int64_t>(a.c.kv_len[seq]) - a.c.cu_q[seq + 1] + t;
+    if (pos < 0 || pos >= a.max_pos) {
+        if (threadIdx.x == 0) record_error(a.c.status, DEV_BAD_INDEX);
+        return;
+    }
+    int64_t page = -1;
+    const int64_t slot = pos >> a.c.page_shift;
+    if (slot < a.c.max_pages) page = a.c.table[seq * a.c.max_pages + slot];
+    const bool held = page >= 0 && page < a.c.num_pages;
+    if (!held && threadIdx.x == 0) record_error(a.c.status, DEV_BAD_INDEX);
+    const int d = (threadIdx.x % kChunks) * 8;
+    float c0[8], c1[8], s0[8], s1[8];
+    load8(a.cos_t + pos * kHd + d, a.vec_table, c0);
+    load8(a.cos_t + pos * kHd + d + kHalf, a.vec_table, c1);
+    load8(a.sin_t + pos * kHd + d, a.vec_table, s0);
+    load8(a.sin_t + pos * kHd + d + kHalf, a.vec_table, s1);
+    const int nh = a.c.nh, nkv = a.c.nkv, all = held ? nh + 2 * nkv : nh;
+    const int64_t in_page = (pos & ((1ll << a.c.page_shift) - 1)) * kHd + d;
+    for (int h = threadIdx.x / kChunks + static_cast<int>(blockIdx.y) * kHeads; h < all;
+         h += kHeads * static_cast<int>(gridDim.y)) {
+        const In* src = h < nh ? static_cast<const In*>(a.q) + t * a.q_stride + h * kHd
+                        : h < nh + nkv ? static_cast<const In*>(a.k) + t * a.k_stride + (h - nh) * kHd
+                                       : static_cast<const In*>(a.v) + t * a.v_stride + (h - nh - nkv) * kHd;
+        float x0[8], x1[8];
+        load8(src + d, a.vec_in, x0);
+        load8(src + d + kHalf, a.vec_in, x1);
+        if (h < nh + nkv) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float lo = __fsub_rn(__fmul_rn(x0[i], c0[i]), __fmul_rn(x1[i], s0[i]));
+                x1[i] = __fadd_rn(__fmul_rn(x1[i], c1[i]), __fmul_rn(x0[i], s1[i]));
+                x0[i] = lo;
+            }
+        }
+        Cache* dst;
+        bool vec = a.vec_cache;
+        if (h < nh) {
+            dst = static_cast<Cache*>(a.q_out) + (t * nh + h) * kHd + d;
+            vec = a.vec_qout;
+        } else {
+            const int hk = h < nh + nkv ? h - nh : h - nh - nkv;
+            dst = static_cast<Cache*>(h < nh + nkv ? a.kp : a.vp) + page * a.c.page_stride +
+                  (static_cast<int64_t>(hk) << a.c.page_shift) * kHd + in_page;
+        }
+        store8(dst, vec, x0);
+        store8(dst + kHalf, vec, x1);
+    }
+}
+
+// ---------------------------------------------------------------- attention, the plain kernel
+// One warp per (token, query head): keys one after the other with a running maximum and sum, each
+// lane holding hd / 32 elements of q and o.
+template <typename T, typename Out, int kHd>
+__global__ void __launch_bounds__(256) k_paged_attn_plain(const T* __restrict__ q, int64_t q_stride, PagedKv c,
+                                                          int64_t max_q, float scale, Out* __restrict__ out,
+                                                          float* __restrict__ lse) {
+    constexpr int kE = kHd / 32;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t item = blockIdx.x * 8ll + (threadIdx.x >> 5);
+    const int64_t t = item / c.nh;
+    const int h = static_cast<int>(item % c.nh);
+    if (t >= c.tokens) return;
+    int seq = 0;
+    for (int b0 = 0; b0 < c.num_seqs; b0 += 32) {
+        const bool before = b0 + lane < c.num_seqs && c.cu_q[b0 + lane + 1] <= t;
+        seq += __popc(__ballot_sync(0xffffffffu, before));
+    }
+    if (seq >= c.num_seqs || t < c.cu_q[seq]) return;
+    const PagedSeq s = paged_seq(c, seq, max_q);
+    if (s.q_len == 0) return;
+    const int pos = s.kv_len - s.q_len + static_cast<int>(t - s.row0);
+    float qf[kE], o[kE] = {};
+#pragma unroll
+    for (int e = 0; e < kE; ++e) qf[e] = to_f32(q[t * q_stride + h * kHd + lane + 32 * e]);
+    float m = -INFINITY, l = 0.0f;
+    const int hk = h / (c.nh / c.nkv);
+    for (int j = 0; j <= pos; ++j) {
+        const int64_t page = c.table[seq * c.max_pages + (j >> c.page_shift)];
+        if (page < 0 || page >= c.num_pages) {
+            record_error(c.status, DEV_BAD_INDEX);
+            continue;
+        }
+        const int64_t at = page * c.page_stride +
+                           ((static_cast<int64_t>(hk) << c.page_shift) + (j & ((1 << c.page_shift) - 1))) * kHd + lane;
+        float d = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) d += qf[e] * to_f32(static_cast<const T*>(c.k)[at + 32 * e]);
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+        d *= scale;
+        const float mn = fmaxf(m, d), f = expf(m - mn), p = expf(d - mn);
+        l = l * f + p;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] = o[e] * f + p * to_f32(static_cast<const T*>(c.v)[at + 32 * e]);
+        m = mn;
+    }
+#pragma unroll
+    for (int e = 0; e < kE; ++e)
+        out[(t * c.nh + h) * kHd + lane + 32 * e] = from_f32<Out>(l > 0.0f ? o[e] / l : 0.0f);
+    if (lse && lane == 0) lse[t * c.nh + h] = l > 0.0f ? m + logf(l) : -INFINITY;
+}
+
+template <typename T, typename Out>
+static cudaError_t launch_plain(const void* q, int64_t q_stride, const PagedKv& c, int hd, int64_t max_q, float scale,
+                                void* out, float* lse, cudaStream_t s) {
+    const dim3 grid(static_cast<unsigned>((c.tokens * c.nh + 7) / 8));
+    return hd == 128 ? launch_pdl(k_paged_attn_plain<T, Out, 128>, grid, dim3(256), 0, s, static_cast<const T*>(q),
+                                  q_stride, c, max_q, scale, static_cast<Out*>(out), lse)
+                     : launch_pdl(k_paged_attn_plain<T, Out, 64>, grid, dim3(256), 0, s, static_cast<const T*>(q),
+                                  q_stride, c, max_q, scale, static_cast<Out*>(out), lse);
+}
+
+template <typename In, typename Cache>
+static cudaError_t launch_append(const AppendArgs& a, int hd, cudaStream_t s) {
+    const int heads_at_once = kAppendThreads / (hd / 16), heads = a.c.nh + 2 * a.c.nkv;
+    // few tokens: the heads of one on several CTAs, down to one pass over them
+    int split = 1;
+    while (a.c.tokens * split < 296 && split * heads_at_once < heads) ++split;
+    const dim3 grid(static_cast<unsigned>(a.c.tokens), static_cast<unsigned>(split));
+    return hd == 128 ? launch_pdl(k_paged_append<In, Cache, 128>, grid, dim3(kAppendThreads), 0, s, a)
+                     : launch_pdl(k_paged_append<In, Cache, 64>, grid, dim3(kAppendThreads), 0, s, a);
+}
+
+static int64_t elem_size(int dtype) { return dtype == SC_F32 ? 4 : 2; }
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+static sc_status paged_bad(const char* who, const char* what) {
+    set_error(std::string(who) + ": " + what);
+    return SC_EINVAL;
+}
+
+// The arguments both entry points share.
+static sc_status make_paged(const char* who, const void* k, const void* v, int dtype, int64_t num_pages, int64_t page_stride,
+                            int page_size, const int32_t* table, int64_t max_pages, const int32_t* cu_q,
+                            const int32_t* kv_len, int64_t num_seqs, int64_t tokens, int nh, int nkv, int hd,
+                            uint32_t* status, PagedKv* c) {
+    if (dtype != SC_F32 && dtype != SC_F16 && dtype != SC_BF16) return paged_bad(who, "the cache is f32, f16 or bf16");
+    if (!k || !v || !table || !cu_q || !kv_len) return paged_bad(who, "null pages, block table or lengths");
+    if (hd != 64 && hd != 128) return paged_bad(who, "head_dim is 64 or 128");
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > kPagedMaxGroup || nh > 65536)
+        return paged_bad(who, "num_heads must be a multiple of num_kv_heads, at most 64 per KV head");
+    if (page_size < kPagedMinPage || page_size > kPagedMaxPage || (page_size & (page_size - 1)))
+        return paged_bad(who, "page_size must be a power of two in 8..256");
+    if (num_pages <= 0 || num_pages > 0x7fffffff || page_stride < static_cast<int64_t>(nkv) * page_size * hd)
+        return paged_bad(who, "pages overlap, or none");
+    if (max_pages <= 0 || max_pages * page_size > 0x7fffffff) return paged_bad(who, "max_pages out of range");
+    if (num_seqs <= 0 || num_seqs > (1 << 20) || tokens > 0x7fffffff / nh)
+        return paged_bad(who, "too many sequences or tokens");
+    const uintptr_t size = static_cast<uintptr_t>(elem_size(dtype));
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % size)
+        return paged_bad(who, "pages must be aligned to their type");
+    c->k = k;
+    c->v = v;
+    c->num_pages = num_pages;
+    c->page_stride = page_stride;
+    c->page_shift = 0;
+    while ((1 << c->page_shift) < page_size) ++c->page_shift;
+    c->table = table;
+    c->max_pages = max_pages;
+    c->cu_q = cu_q;
+    c->kv_len = kv_len;
+    c->num_seqs = static_cast<int>(num_seqs);
+    c->tokens = tokens;
+    c->nh = nh;
+    c->nkv = nkv;
+    c->status = status;
+    return SC_OK;
+}
+
+}  // namespace sc
+
+using namespace sc;
+
+extern "C" {
+
+sc_status sc_qwen2_paged_append(const void* q, const void* k, const void* v, int in_dtype, int64_t q_stride,
+                                int64_t k_stride, int64_t v_stride, int64_t tokens, const float* cos_table,
+                                const float* sin_table, int64_t max_pos, int num_heads, int num_kv_heads, int head_dim,
+                                void* k_pages, void* v_pages, int cache_dtype, int64_t num_pages, int64_t page_stride,
+                                int page_size, const int32_t* block_table, int64_t max_pages, const int32_t* cu_q,
+                                const int32_t* kv_len, int64_t num_seqs, void* q_out, uint32_t* status, void* stream) {
+    const char* who = "sc_qwen2_paged_append";
+    if (tokens <= 0) return tokens == 0 ? SC_OK : paged_bad(who, "a negative number of tokens");
+    AppendArgs a = {};
+    const sc_status st = make_paged(who, k_pages, v_pages, cache_dtype, num_pages, page_stride, page_size, block_table,
+                                    max_pages, cu_q, kv_len, num_seqs, tokens, num_heads, num_kv_heads, head_dim,
+                                    status, &a.c);
+    if (st != SC_OK) return st;
+    if (!q || !k || !v || !q_out || !cos_table || !sin_table) return paged_bad(who, "null q, k, v, q_out or table");
+    if (in_dtype != SC_F32 && in_dtype != cache_dtype) return paged_bad(who, "q, k and v are f32 or of the cache's type");
+    if (max_pos <= 0) return paged_bad(who, "empty rotation tables");
+    const int64_t qw = static_cast<int64_t>(num_heads) * head_dim, kw = static_cast<int64_t>(num_kv_heads) * head_dim;
+    if (tokens > 1 && (q_stride < qw || k_stride < kw || v_stride < kw)) return paged_bad(who, "rows overlap");
+    if (q_out == q && (in_dtype != cache_dtype || (tokens > 1 && q_stride != qw)))
+        return paged_bad(who, "in place needs contiguous rows of the cache's type");
+    const int64_t is = elem_size(in_dtype), cs = elem_size(cache_dtype);
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % is ||
+        reinterpret_cast<uintptr_t>(q_out) % cs ||
+        (reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) % 4)
+        return paged_bad(who, "tensors must be aligned to their type");
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.cos_t = cos_table;
+    a.sin_t = sin_table;
+    a.max_pos = max_pos;
+    a.kp = k_pages;
+    a.vp = v_pages;
+    a.q_out = q_out;
+    a.vec_in = aligned16(q) && aligned16(k) && aligned16(v) && (q_stride * is | k_stride * is | v_stride * is) % 16 == 0;
+    a.vec_cache = aligned16(k_pages) && aligned16(v_pages) && page_stride * cs % 16 == 0;
+    a.vec_table = aligned16(cos_table) && aligned16(sin_table);
+    a.vec_qout = aligned16(q_out);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e =
+        cache_dtype == SC_F32 ? launch_append<float, float>(a, head_dim, s)
+        : cache_dtype == SC_F16
+            ? (in_dtype == SC_F32 ? launch_append<float, __half>(a, head_dim, s) : launch_append<__half, __half>(a, head_dim, s))
+            : (in_dtype == SC_F32 ? launch_append<float, __nv_bfloat16>(a, head_dim, s)
+                                  : launch_append<__nv_bfloat16, __nv_bfloat16>(a, head_dim, s));
+    return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
+}
+
+size_t sc_qwen2_paged_attention_scratch(int64_t tokens, int64_t num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                        int64_t max_q_len, int cache_dtype) {
+    (void)tokens, (void)num_seqs, (void)num_heads, (void)num_kv_heads, (void)head_dim, (void)max_q_len, (void)cache_dtype;
+    return 0;
+}
+
+sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                                   int cache_dtype, int64_t num_pages, int64_t page_stride, int page_size,
+                                   const int32_t* block_table, int64_t max_pages, const int32_t* cu_q,
+                                   const int32_t* kv_len, int64_t num_seqs, int64_t tokens, int num_heads,
+                                   int num_kv_heads, int head_dim, int64_t max_q_len, int64_t max_kv_len, float scale,
+                                   void* out, int out_dtype, float* lse, void* scratch, size_t scratch_bytes,
+                                   uint32_t* status, void* stream) {
+    const char* who = "sc_qwen2_paged_attention";
+    if (tokens <= 0) return tokens == 0 ? SC_OK : paged_bad(who, "a negative number of tokens");
+    PagedKv c;
+    const sc_status st = make_paged(who, k_pages, v_pages, cache_dtype, num_pages, page_stride, page_size, block_table,
+                                    max_pages, cu_q, kv_len, num_seqs, tokens, num_heads, num_kv_heads, head_dim,
+                                    status, &c);
+    if (st != SC_OK) return st;
+    if (!q || !out) return paged_bad(who, "null q or out");
+    if (out_dtype != cache_dtype && !(cache_dtype == SC_F32 && out_dtype == SC_F16))
+        return paged_bad(who, "out is of the cache's type, or f16 from an f32 cache");
+    if (max_q_len <= 0 || max_kv_len <= 0) return paged_bad(who, "max_q_len and max_kv_len must be positive");
+    if (!(scale == scale) || scale - scale != 0.0f) return paged_bad(who, "scale must be finite");
+    const int64_t cs = elem_size(cache_dtype);
+    if (tokens > 1 && q_stride < static_cast<int64_t>(num_heads) * head_dim) return paged_bad(who, "rows of q overlap");
+    if (!aligned16(q) || (tokens > 1 && q_stride * cs % 16) || !aligned16(k_pages) || !aligned16(v_pages) ||
+        page_stride * cs % 16 || !aligned16(out))
+        return paged_bad(who, "q, the pages, their strides and out must be 16-byte aligned");
+    if (scratch_bytes < sc_qwen2_paged_attention_scratch(tokens, num_seqs, num_heads, num_kv_heads, head_dim, max_q_len,
+                                                         cache_dtype)) {
+        set_error(std::string(who) + ": scratch too small");
+        return SC_ENOMEM;
+    }
+    (void)scratch;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e =
+        cache_dtype == SC_F16 ? launch_plain<__half, __half>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s)
+        : cache_dtype == SC_BF16
+            ? launch_plain<__nv_bfloat16, __nv_bfloat16>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s)
+        : out_dtype == SC_F16 ? launch_plain<float, __half>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s)
+                              : launch_plain<float, float>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s);
+    return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
+}
+
+}  // extern "C"

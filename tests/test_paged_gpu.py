@@ -1,0 +1,309 @@
+"""The paged cache on the GPU: appending and attention against a plain implementation in 64 bits."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from paged_cases import U, Paged
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def sc():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    import saccade_core
+    return saccade_core
+
+
+def attend(sc, c, **kw):
+    out = torch.full((c.tokens, c.nh, c.hd), 7.0, dtype=kw.pop("out_dtype", c.dtype), device=c.q.device)
+    status = torch.zeros(1, dtype=torch.int32, device=c.q.device)
+    got, lse = sc.paged_attention(c.q, c.k_pages, c.v_pages, c.table, c.cu_q, c.kv_len, c.max_q, c.max_kv, out=out,
+                                  return_lse=True, status=status, **kw)
+    torch.cuda.synchronize()
+    assert got is out and int(status.item()) == 0
+    return got, lse
+
+
+def compare(c, got, lse, scale):
+    ref, rl, tol, ltol = c.attention(scale)
+    end = c.cu[-1]
+    err = (got[:end].cpu().double() - ref[:end]).abs()
+    assert torch.isfinite(got[:end]).all()
+    assert (err <= tol[:end]).all(), float((err / tol[:end].clamp(min=1e-300)).max())
+    assert (got[end:] == 7.0).all(), "rows behind the last sequence are left as they were"
+    empty = rl[:end] == -math.inf
+    assert torch.equal(lse[:end].cpu() == -math.inf, empty)
+    lerr = torch.where(empty, 0.0, (lse[:end].cpu().double() - rl[:end]).abs().nan_to_num(0.0))
+    assert (lerr <= ltol[:end]).all()
+
+
+LENS = {
+    "decode": [(1, n) for n in (1, 2, 7, 8, 15, 16, 17, 63, 64, 65, 127, 128, 129, 200, 255, 257, 300)],
+    "decode-long": [(1, 4096), (1, 3001), (1, 1), (1, 2047)],
+    "ragged": [(1, 100), (0, 50), (33, 33), (2, 2), (130, 200), (1, 1), (0, 0), (64, 300), (17, 1000)],
+    "chunk": [(300, 1111), (257, 257)],
+    "short": [(2, 70), (5, 5), (3, 400), (4, 129)],
+    "one": [(1, 1)],
+    "none": [(0, 0), (0, 12)],
+}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (3, 1, 128), (8, 8, 64), (16, 2, 128), (20, 1, 64)],
+                         ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("lens", list(LENS), ids=list(LENS))
+def test_attention_matches_64_bits(sc, dtype, heads, lens):
+    page = {"decode": 16, "decode-long": 64, "ragged": 8, "chunk": 32, "short": 128, "one": 256, "none": 8}[lens]
+    c = Paged(LENS[lens], *heads, page, dtype, "cuda", seed=len(lens) + heads[0], behind=3)
+    scale = heads[2] ** -0.5
+    compare(c, *attend(sc, c), scale)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
+def test_attention_page_sizes_strides_and_bounds(sc, dtype, page):
+    """Pages that end inside a tile, pages apart from one another, q as a slice of a wider buffer, a
+    scale of its own, and length bounds far above the lengths."""
+    c = Paged([(1, 37), (40, 513), (1, 1000), (9, 9)], 14, 2, 64, page, dtype, "cuda", seed=page, behind=1, gap=64)
+    wide = torch.full((c.tokens, 18, 64), math.nan, dtype=dtype, device="cuda")
+    wide[:, :14] = c.q
+    c.q = wide[:, :14]
+    c.max_q, c.max_kv = c.tokens, 1 << 20
+    compare(c, *attend(sc, c, scale=0.3), 0.3)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+def test_attention_extreme_scores(sc, dtype):
+    """Scores of hundreds: weights from 1 down to zero, maxima that move by more than any exponent."""
+    c = Paged([(1, 700), (150, 400)], 8, 2, 128, 32, dtype, "cuda", seed=5, scale=6.0)
+    compare(c, *attend(sc, c), 128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+def test_negative_positions_attend_nothing(sc, dtype):
+    """More new tokens than positions: the first rows' positions are negative and attend no key."""
+    c = Paged([(5, 2), (1, 9), (200, 150), (1, 0), (3, 0)], 14, 2, 64, 16, dtype, "cuda", seed=9, behind=2)
+    got, lse = attend(sc, c)
+    compare(c, got, lse, 0.125)
+    assert (got[:3] == 0).all() and (lse[:3] == -math.inf).all() and (got[c.cu[3]:c.cu[5]] == 0).all()
+
+
+def test_f32_cache_to_f16_output(sc):
+    c = Paged([(1, 300), (20, 77)], 14, 2, 64, 16, F32, "cuda", seed=3)
+    full, _ = attend(sc, c)
+    half, _ = attend(sc, c, out_dtype=F16)
+    assert torch.equal(half, full.to(F16))
+
+
+@pytest.mark.parametrize("lens", ["decode", "chunk"])
+def test_two_calls_are_the_same_bits_and_streams_do_not_mix(sc, lens):
+    c = Paged(LENS[lens], 28, 4, 128, 16, BF16, "cuda", seed=1)
+    d = Paged(LENS[lens], 28, 4, 128, 16, BF16, "cuda", seed=2)
+    a0, b0 = attend(sc, c)[0], attend(sc, d)[0]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        with torch.cuda.stream(s1):
+            a = sc.paged_attention(c.q, c.k_pages, c.v_pages, c.table, c.cu_q, c.kv_len, c.max_q, c.max_kv)
+        with torch.cuda.stream(s2):
+            b = sc.paged_attention(d.q, d.k_pages, d.v_pages, d.table, d.cu_q, d.kv_len, d.max_q, d.max_kv)
+    torch.cuda.synchronize()
+    assert torch.equal(a, a0) and torch.equal(b, b0)
+
+
+def test_attention_in_a_graph_follows_lengths_and_tables(sc):
+    """A captured call replays with other lengths and pages in the same tensors."""
+    c = Paged([(1, 40), (1, 500), (1, 3)], 14, 2, 64, 16, F16, "cuda", seed=11)
+    d = Paged([(1, 333), (1, 1), (1, 511)], 14, 2, 64, 16, F16, "cuda", seed=12)
+    width = max(c.table.shape[1], d.table.shape[1])
+    table = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+    pages = max(c.pages, d.pages)
+    kp = torch.full((pages, 2, 16, 64), math.nan, dtype=F16, device="cuda")
+    vp, q, kv, cu = kp.clone(), torch.empty_like(c.q), c.kv_len.clone(), c.cu_q.clone()
+
+    def fill(x):
+        table.fill_(-1)[:, :x.table.shape[1]] = x.table
+        kp[:x.pages], vp[:x.pages] = x.k_pages, x.v_pages
+        q.copy_(x.q), kv.copy_(x.kv_len)
+
+    fill(c)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        sc.paged_attention(q, kp, vp, table, cu, kv, 1, 512)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = sc.paged_attention(q, kp, vp, table, cu, kv, 1, 512)
+    for x in (c, d, c):
+        fill(x)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = sc.paged_attention(x.q, x.k_pages, x.v_pages, x.table, x.cu_q, x.kv_len, 1, 512)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_bad_pages_and_lengths_are_recorded_and_not_followed(sc, dtype, q_len):
+    c = Paged([(q_len, 100), (q_len, 60), (q_len, 90)], 14, 2, 64, 16, dtype, "cuda", seed=4)
+    good, _ = attend(sc, c)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def again():
+        status.zero_()
+        out = torch.full_like(good, 7.0)
+        sc.paged_attention(c.q, c.k_pages, c.v_pages, c.table, c.cu_q, c.kv_len, c.max_q, c.max_kv, out=out, status=status)
+        torch.cuda.synchronize()
+        return out, int(status.item())
+
+    assert again()[1] == 0
+    for bad in (-1, c.pages, 2**31 - 1, -2**31):
+        keep = int(c.table[1, 2])
+        c.table[1, 2] = bad
+        out, st = again()
+        assert st != 0 and torch.equal(out[:q_len], good[:q_len]) and torch.equal(out[2 * q_len:], good[2 * q_len:])
+        c.table[1, 2] = keep
+    for bad in (c.table.shape[1] * 16 + 1, 2**31 - 1, -5):
+        c.kv_len[1] = bad
+        out, st = again()
+        assert st != 0 and (out[q_len:2 * q_len] == 7.0).all()
+        assert torch.equal(out[:q_len], good[:q_len]) and torch.equal(out[2 * q_len:], good[2 * q_len:])
+        c.kv_len[1] = 60
+    # a sequence of more new tokens than the bound, one that reaches behind the rows
+    c.max_q = q_len - 1 if q_len > 1 else 1
+    if q_len > 1:
+        out, st = again()
+        assert st != 0 and (out == 7.0).all()
+    c.max_q = q_len
+    keep = c.cu_q.clone()
+    c.cu_q[3] = c.tokens + 1
+    out, st = again()
+    assert st != 0 and torch.equal(out[:2 * q_len], good[:2 * q_len]) and (out[2 * q_len:] == 7.0).all()
+    c.cu_q.copy_(keep)
+    assert torch.equal(again()[0], good)
+
+
+# ---------------------------------------------------------------- append
+
+
+def tables(n, hd, device):
+    ang = torch.arange(n, dtype=torch.float64)[:, None] * (1.0e6 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd))
+    ang = torch.cat([ang, ang], 1)
+    return ang.cos().float().to(device), ang.sin().float().to(device)
+
+
+@pytest.mark.parametrize("src,dtype", [(F32, F16), (F32, BF16), (F32, F32), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (3, 1, 128), (64, 8, 128)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("layout", ["apart", "fused", "odd"])
+def test_append_matches_64_bits(sc, src, dtype, heads, layout):
+    nh, nkv, hd = heads
+    lens = [(1, 1), (5, 40), (0, 30), (1, 17), (70, 70), (3, 129)]
+    c = Paged(lens, nh, nkv, hd, 16, dtype, "cuda", seed=nh, behind=2, gap=8 if layout == "odd" else 0)
+    g = torch.Generator("cuda").manual_seed(1)
+    extra = 1 if layout == "odd" else 0  # rows that start off any 16-byte boundary
+    buf = torch.randn(c.tokens, (nh + 2 * nkv) * hd + extra, device="cuda", generator=g).to(src)
+    q, k, v = (buf[:, a * hd:b * hd].unflatten(1, (b - a, hd)) for a, b in ((0, nh), (nh, nh + nkv), (nh + nkv, nh + 2 * nkv)))
+    if layout == "apart":
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    cos, sin = tables(130, hd, "cuda")
+    kp, vp = c.k_pages.clone(), c.v_pages.clone()
+    if layout == "odd":
+        kp, vp = c.k_pages, c.v_pages
+    before_k, before_v = kp.clone(), vp.clone()
+    out = torch.full((c.tokens, nh, hd), 7.0, dtype=dtype, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = sc.paged_append(q, k, v, cos, sin, kp, vp, c.table, c.cu_q, c.kv_len, out=out, status=status)
+    torch.cuda.synchronize()
+    assert got is out and int(status.item()) == 0
+    want_k, want_v, u = before_k.double(), before_v.double(), U[dtype]
+    tol_k = torch.zeros_like(want_k)
+    for b, (n, kv) in enumerate(lens):
+        rows, pos = slice(c.cu[b], c.cu[b + 1]), torch.arange(kv - n, kv, device="cuda")
+        if n == 0:
+            continue
+        cs, sn = cos[pos][:, None].double(), sin[pos][:, None].double()
+        sign = torch.cat([-torch.ones(hd // 2), torch.ones(hd // 2)]).double().cuda()
+        rot = lambda t: t.double() * cs + t.double().roll(hd // 2, -1) * sign * sn  # noqa: E731
+        # two products and their sum, each rounded in f32, then one rounding to the cache's type
+        mag = lambda t: (t.double() * cs).abs() + (t.double().roll(hd // 2, -1) * sn).abs()  # noqa: E731
+        tol = lambda t: mag(t) * 2.0 ** -23 + u * rot(t).abs() * 1.001 + (2.0 ** -25 if dtype == F16 else 0)  # noqa: E731
+        assert ((out[rows].double() - rot(q[rows])).abs() <= tol(q[rows])).all()
+        page = c.table[b].long()[pos // 16]
+        want_k[page, :, pos % 16], want_v[page, :, pos % 16] = rot(k[rows]), v[rows].to(dtype).double()
+        tol_k[page, :, pos % 16] = tol(k[rows])
+    assert (out[c.cu[-1]:] == 7.0).all()
+    same = torch.isnan(want_k) & torch.isnan(kp.double())
+    assert (same | ((kp.double() - want_k).abs() <= tol_k)).all()
+    assert torch.equal(vp.double().nan_to_num(99.0), want_v.nan_to_num(99.0))
+    if src == dtype and layout == "apart":  # in place: the same bits
+        sc.paged_append(q, k, v, cos, sin, kp, vp, c.table, c.cu_q, c.kv_len, out=q)
+        assert torch.equal(q[:c.cu[-1]], out[:c.cu[-1]])
+
+
+def test_append_skips_what_has_no_place(sc):
+    c = Paged([(2, 20), (1, 33), (2, 1), (1, 5)], 14, 2, 64, 16, F16, "cuda", seed=8)
+    q, k, v = (torch.randn(c.tokens, n, 64, device="cuda") for n in (14, 2, 2))
+    cos, sin = tables(40, 64, "cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def run():
+        kp, vp = torch.full_like(c.k_pages, 3.0), torch.full_like(c.v_pages, 3.0)
+        out = torch.full((c.tokens, 14, 64), 7.0, dtype=F16, device="cuda")
+        status.zero_()
+        sc.paged_append(q, k, v, cos, sin, kp, vp, c.table, c.cu_q, c.kv_len, out=out, status=status)
+        torch.cuda.synchronize()
+        return out, kp, vp, int(status.item())
+
+    out, kp, vp, st = run()  # sequence 2 has one position for two tokens: the first has none
+    assert st != 0 and (out[3] == 7.0).all() and not (out[4] == 7.0).any()
+    c.kv_len[2] = 2
+    out, kp, vp, st = run()
+    assert st == 0
+    for bad in (-1, c.pages, 2**31 - 1):
+        keep = int(c.table[1, 2])
+        c.table[1, 2] = bad  # position 32's page
+        out2, kp2, vp2, st = run()
+        assert st != 0 and torch.equal(out2, out)
+        assert (kp2[keep] == 3.0).all() and (vp2[keep] == 3.0).all()
+        kp2[keep], vp2[keep] = kp[keep], vp[keep]
+        assert torch.equal(kp2, kp) and torch.equal(vp2, vp)
+        c.table[1, 2] = keep
+    for bad in (41, 10**6, 2**31 - 1, -3):  # beyond the rotation tables, and the block table, and before 0
+        c.kv_len[3] = bad
+        out2, _, _, st = run()
+        assert st != 0 and (out2[5] == 7.0).all() and torch.equal(out2[:5], out[:5])
+        c.kv_len[3] = 5
+    assert run()[3] == 0
+
+
+def test_append_then_attend_is_one_prefill(sc):
+    """A prompt appended and attended in chunks of any size gives what one pass gives, within the
+    rounding of a few keys' order (f32), and decoding continues it."""
+    nh, nkv, hd, page, n = 14, 2, 64, 16, 203
+    g = torch.Generator("cuda").manual_seed(2)
+    q, k, v = (torch.randn(n, h, hd, device="cuda", generator=g) for h in (nh, nkv, nkv))
+    cos, sin = tables(n, hd, "cuda")
+    table = torch.randperm(16, device="cuda", generator=g)[None].to(torch.int32)
+
+    def run(cuts):
+        kp, vp = torch.zeros(16, nkv, page, hd, device="cuda"), torch.zeros(16, nkv, page, hd, device="cuda")
+        outs = []
+        for a, b in zip([0] + cuts, cuts + [n]):
+            cu = torch.tensor([0, b - a], dtype=torch.int32, device="cuda")
+            kv = torch.tensor([b], dtype=torch.int32, device="cuda")
+            qr = sc.paged_append(q[a:b], k[a:b], v[a:b], cos, sin, kp, vp, table, cu, kv)
+            outs.append(sc.paged_attention(qr, kp, vp, table, cu, kv, b - a, n))
+        return torch.cat(outs), kp, vp
+
+    whole, kp, vp = run([])
+    for cuts in ([1], [64, 128], [100, 101, 102, 150], list(range(180, n))):
+        part, kp2, vp2 = run(cuts)
+        assert torch.equal(kp, kp2) and torch.equal(vp, vp2)
+        assert (part - whole).abs().max() <= 2e-5  # f32 sums of up to 203 terms of size ~1, regrouped
