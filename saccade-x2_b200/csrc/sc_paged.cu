@@ -1,6 +1,9 @@
 // sc_paged.cu -- the paged KV cache: rotation and appending of new tokens, and causal attention of the
 // new tokens over the pages.
+#include <cudaTypedefs.h>
+
 #include <atomic>
+#include <mutex>
 #include <string>
 
 #include "saccade_qwen2.h"
@@ -217,6 +220,61 @@ static cudaError_t launch_append(const AppendArgs& a, int hd, cudaStream_t s) {
                      : launch_pdl(k_paged_append<In, Cache, 64>, grid, dim3(kAppendThreads), 0, s, a);
 }
 
+static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static std::once_flag once;
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+cudaError_t paged_tensor_map(CUtensorMap* map, const PagedKv& c, const void* pages, int dtype, int hd, int box_rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t page = 1ull << c.page_shift;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), page, static_cast<cuuint64_t>(c.nkv),
+                                static_cast<cuuint64_t>(c.num_pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(hd) * 2, page * hd * 2,
+                                   static_cast<cuuint64_t>(c.page_stride) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, dtype == SC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                              const_cast<void*>(pages), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+static int sm_count() {
+    static std::atomic<int> cache[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if ((n = cache[dev].load()) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    cache[dev].store(n);
+    return n;
+}
+
+// The kernel of a call and its work division.
+struct PagedPlan {
+    bool decode;           // the 16-row kernel
+    int ctas;
+    PagedTiling tl;
+};
+static PagedPlan paged_plan(int dtype, int nh, int nkv, int64_t max_q) {
+    PagedPlan p{};
+    const int G = nh / nkv;
+    p.decode = dtype != SC_F32 && max_q * G <= 16;
+    p.ctas = 2 * sm_count();
+    p.tl = PagedTiling{16, 16, G <= 16 ? 16 / G : 1, 64};
+    return p;
+}
+
 static int64_t elem_size(int dtype) { return dtype == SC_F32 ? 4 : 2; }
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -322,8 +380,10 @@ sc_status sc_qwen2_paged_append(const void* q, const void* k, const void* v, int
 
 size_t sc_qwen2_paged_attention_scratch(int64_t tokens, int64_t num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                         int64_t max_q_len, int cache_dtype) {
-    (void)tokens, (void)num_seqs, (void)num_heads, (void)num_kv_heads, (void)head_dim, (void)max_q_len, (void)cache_dtype;
-    return 0;
+    (void)tokens, (void)num_seqs;
+    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || max_q_len <= 0) return 0;
+    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, max_q_len);
+    return p.decode ? paged_scratch_bytes(p.ctas, p.tl.rows, head_dim) : 0;
 }
 
 sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
@@ -355,8 +415,16 @@ sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* 
         set_error(std::string(who) + ": scratch too small");
         return SC_ENOMEM;
     }
-    (void)scratch;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, max_q_len);
+    if (p.decode) {
+        if (!scratch || !aligned16(scratch)) return paged_bad(who, "scratch must be 16-byte aligned");
+        const PagedLaunch a{c, q, q_stride, max_q_len, {out, lse, scale * 1.4426950408889634f}, p.tl,
+                            paged_scratch(scratch, p.ctas, p.tl.rows, head_dim)};
+        cudaError_t e = launch_paged_decode(a, cache_dtype, head_dim, p.ctas, s);
+        if (e == cudaSuccess) e = launch_paged_combine(a, out_dtype, head_dim, p.ctas, s);
+        return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
+    }
     const cudaError_t e =
         cache_dtype == SC_F16 ? launch_plain<__half, __half>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s)
         : cache_dtype == SC_BF16

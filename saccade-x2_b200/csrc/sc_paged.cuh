@@ -1,9 +1,12 @@
 // sc_paged.cuh -- the paged KV cache as the kernels see it.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+
+#include <atomic>
 
 #include "sc_device.cuh"
 #include "sc_internal.h"
@@ -52,5 +55,230 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedKv& p, int b, int64_t m
     }
     return s;
 }
+
+// ---------------------------------------------------------------- work division
+// An item is a (sequence, KV head, row tile): tt consecutive new tokens with all query heads of the
+// KV head, over key tiles of kt positions 0 .. (the row tile's last position).  The key tiles of all
+// items, sequences first, then KV heads, then row tiles, form one line that is cut into equal pieces,
+// one per CTA: no CTA has more than one tile above the mean whatever the lengths are.  An item cut by a
+// piece's border leaves partial results (unnormalised output, maximum, sum) in the scratch, one slot
+// for the item that the CTA continues (0) and one for the item that it begins and does not finish (1);
+// k_paged_combine joins them in order.
+struct PagedCut {
+    int64_t total, per;    // tiles in all, tiles per CTA
+    int64_t first, left;   // this CTA's first tile and number of tiles
+    int b, h, rt, tile;    // where the first one is
+};
+
+__device__ __forceinline__ int paged_row_tiles(const PagedSeq& s, int tt) { return (s.q_len + tt - 1) / tt; }
+
+// Key tiles of row tile rt: at least one, so that rows without a key get their zeros.
+__device__ __forceinline__ int paged_key_tiles(const PagedSeq& s, int rt, int tt, int kt) {
+    const int last = min((rt + 1) * tt, s.q_len);
+    const int keys = s.kv_len - s.q_len + last;
+    return keys <= kt ? 1 : (keys + kt - 1) / kt;
+}
+
+__device__ __forceinline__ int64_t paged_seq_tiles(const PagedSeq& s, int tt, int kt) {
+    int64_t n = 0;
+    const int rts = paged_row_tiles(s, tt);
+    for (int rt = 0; rt < rts; ++rt) n += paged_key_tiles(s, rt, tt, kt);
+    return n;
+}
+
+// The piece of CTA blockIdx.x of gridDim.x; every thread of the block calls it.
+template <int kThreads>
+__device__ __forceinline__ void paged_cut(const PagedKv& p, int64_t max_q, int tt, int kt, PagedCut* cut) {
+    __shared__ int64_t s_warp[kThreads / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // inclusive prefix sums of the sequences' tiles, a block of sequences at a time
+    auto scan = [&](int64_t v, int64_t* block) {
+        int64_t x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) s_warp[warp] = x;
+        __syncthreads();
+        int64_t before = 0, all = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) {
+            if (i < warp) before += s_warp[i];
+            all += s_warp[i];
+        }
+        *block = all;
+        return x + before;
+    };
+    auto tiles = [&](int b) -> int64_t {
+        return b < p.num_seqs ? p.nkv * paged_seq_tiles(paged_seq(p, b, max_q), tt, kt) : 0;
+    };
+    int64_t total = 0, block = 0, mine = 0, incl = 0;
+    for (int b0 = 0; b0 < p.num_seqs; b0 += kThreads) {
+        mine = tiles(b0 + tid);
+        incl = scan(mine, &block);
+        total += block;
+    }
+    const int64_t per = total > 0 ? (total + gridDim.x - 1) / gridDim.x : 1;
+    const int64_t first = per * blockIdx.x;
+    if (tid == 0) {
+        cut->total = total;
+        cut->per = per;
+        cut->first = first;
+        cut->left = first < total ? imin64(per, total - first) : 0;
+    }
+    int64_t base = 0;
+    for (int b0 = 0; b0 < p.num_seqs && first < total; b0 += kThreads) {
+        if (p.num_seqs > kThreads) {
+            mine = tiles(b0 + tid);
+            incl = scan(mine, &block);
+        }
+        const int64_t rel = first - base;
+        if (rel >= incl - mine && rel < incl) {
+            const int b = b0 + tid;
+            const PagedSeq s = paged_seq(p, b, max_q);
+            const int64_t per_head = mine / p.nkv;
+            int64_t at = rel - (incl - mine);
+            cut->b = b;
+            cut->h = static_cast<int>(at / per_head);
+            at %= per_head;
+            int rt = 0;
+            for (int n; at >= (n = paged_key_tiles(s, rt, tt, kt)); ++rt) at -= n;
+            cut->rt = rt;
+            cut->tile = static_cast<int>(at);
+        }
+        base += block;
+    }
+    __syncthreads();
+}
+
+// Walks the items of a piece; every role of a CTA walks them by itself.
+struct PagedWalk {
+    PagedSeq s;
+    int b, h, rt;
+    int tiles;      // key tiles of the item
+    int t0, t1;     // the piece's share of them
+    int64_t at, left;
+    int next_tile;
+
+    __device__ __forceinline__ void begin(const PagedCut& c) {
+        b = c.b;
+        h = c.h;
+        rt = c.rt - 1;
+        next_tile = c.tile;
+        at = c.first;
+        left = c.left;
+        t0 = t1 = tiles = 0;
+        s = PagedSeq{0, 0, 0};
+        fresh = true;
+    }
+    // The next item, or false at the piece's end.
+    __device__ __forceinline__ bool next(const PagedKv& p, int64_t max_q, int tt, int kt) {
+        if (left <= 0) return false;
+        if (fresh) {
+            s = paged_seq(p, b, max_q);
+            fresh = false;
+        }
+        if (++rt >= paged_row_tiles(s, tt)) {
+            rt = 0;
+            if (++h >= p.nkv) {
+                h = 0;
+                do {
+                    if (++b >= p.num_seqs) return false;
+                    s = paged_seq(p, b, max_q);
+                } while (s.q_len == 0);
+            }
+        }
+        tiles = paged_key_tiles(s, rt, tt, kt);
+        t0 = next_tile;
+        t1 = static_cast<int>(imin64(tiles, t0 + left));
+        next_tile = 0;
+        at += t1 - t0;
+        left -= t1 - t0;
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
+    __device__ __forceinline__ int slot() const { return t0 > 0 ? 0 : 1; }
+
+private:
+    bool fresh;
+};
+
+// What k_paged_combine joins: the item that CTA w begins and does not finish (pieces 0: none).
+struct PagedJoin {
+    int64_t row0;          // the sequence's first token row
+    int q_len, h, rt, pieces;
+};
+
+// Scratch of a launch of `ctas` CTAs with row tiles of `rows` rows.
+struct PagedScratch {
+    PagedJoin* join;       // [ctas]
+    float* ml;             // [ctas][2 slots][rows][maximum (log2 units), sum]
+    float* o;              // [ctas][2 slots][rows][hd]
+};
+inline size_t paged_scratch_bytes(int64_t ctas, int rows, int hd) {
+    return static_cast<size_t>(ctas) * (sizeof(PagedJoin) + 2ull * rows * (hd + 2) * 4);
+}
+inline PagedScratch paged_scratch(void* base, int64_t ctas, int rows, int hd) {
+    PagedScratch s;
+    s.o = static_cast<float*>(base);
+    s.ml = s.o + ctas * 2 * rows * hd;
+    s.join = reinterpret_cast<PagedJoin*>(s.ml + ctas * 2 * rows * 2);
+    return s;
+}
+
+// How a launch divides its work.
+struct PagedTiling {
+    int rows;   // rows of a row tile as the kernel holds them (token-major, `group` query heads each)
+    int sub;    // rows per independent half, of which floor(sub / group) * group are used
+    int tt;     // tokens of a row tile
+    int kt;     // positions of a key tile
+};
+
+struct PagedOut {
+    void* out;
+    float* lse;
+    float sl2;             // scale * log2(e)
+};
+
+// Row r of a row tile: its token in the sequence and its query head of the group, or token -1.
+__device__ __forceinline__ int paged_row_token(int r, int sub, int group, int rt, int tt, int q_len, int* g) {
+    const int per = sub / group, half = r / sub, x = r - half * sub;
+    const int tok = x / group;
+    *g = x - tok * group;
+    const int t = rt * tt + half * per + tok;
+    return tok < per && t < q_len ? t : -1;
+}
+
+struct PagedLaunch {
+    PagedKv c;
+    const void* q;
+    int64_t q_stride;
+    int64_t max_q;
+    PagedOut o;
+    PagedTiling tl;
+    PagedScratch sc;
+};
+
+// The pages as a tensor {head_dim, page, KV heads, pages} with boxes of 64 elements x box_rows positions, each
+// box landing as rows of 128 bytes in the 128-byte swizzle (16-bit caches).
+cudaError_t paged_tensor_map(CUtensorMap* map, const PagedKv& c, const void* pages, int dtype, int hd, int box_rows);
+
+// Raises a kernel's dynamic shared-memory limit once per device.
+template <typename Kern>
+cudaError_t paged_allow_smem(Kern kern, std::atomic<uint64_t>& flags, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (flags.load() & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) flags.fetch_or(bit);
+    return e;
+}
+
+cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
+cudaError_t launch_paged_combine(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);
 
 }  // namespace sc

@@ -1,0 +1,462 @@
+// sc_paged_decode.cu -- attention of few new tokens per sequence over the paged cache (16-bit caches).
+//
+// Up to 16 rows (new tokens x query heads of one KV head) share each key and value that is loaded:
+// 4 * 16 flops at most per 2 bytes, so the cache's bytes bound it and the tensor work (mma.sync
+// m16n8k16, under a tenth of its rate) does not.  What counts is that the loads never stop:
+//   producer warp   per key tile of 64 positions, boxes of K and V (min(page, 64) rows x 64 elements,
+//                   128-byte swizzle) by TMA into a ring of stages, two CTAs per SM: ~190 KB in flight
+//   4 warps         each takes 16 of the tile's 64 positions with a running maximum and sum of its own,
+//                   so no warp waits for another until the item ends: S = Q K^T (registers), weights
+//                   p = 2^(s scale log2 e - m) in f32, split into a high and a low 16-bit part
+//                   (P V then has 22 bits of p in f16, 16 in bf16, at no time that shows), O += P V
+//   item end        the 4 warps' maxima, sums and outputs are joined through shared memory.
+// The work is cut evenly over the CTAs along the positions (sc_paged.cuh).
+#include <atomic>
+#include <type_traits>
+
+#include "sc_paged.cuh"
+
+namespace sc {
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+template <typename T>
+struct Mma16;
+template <>
+struct Mma16<__half> {
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        mma_16816(d, a, b0, b1);
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+};
+template <>
+struct Mma16<__nv_bfloat16> {
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void tma_page(void* smem_dst, const CUtensorMap* map, int col, int row, int head, int page,
+                                         uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+template <int kHd>
+struct DecCfg {
+    static constexpr int kKeys = 64;                            // positions of a stage
+    static constexpr int kTile = kKeys * kHd * 2;               // bytes of its K (or V)
+    static constexpr int kStages = kHd == 128 ? 3 : 6;
+    static constexpr int kWarps = 4;
+    static constexpr int kThreads = (kWarps + 1) * 32;
+    static constexpr int kJoinDims = 32;                        // output columns joined at a time
+    static constexpr int kSmem = 1024 + kStages * 2 * kTile + kWarps * 16 * kJoinDims * 4;
+};
+
+struct alignas(64) DecodeParams {
+    CUtensorMap kmap, vmap;
+    PagedLaunch a;
+    int box_shift;         // log2 of the rows of a box
+};
+
+template <typename T, int kHd>
+__global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const __grid_constant__ DecodeParams P) {
+    using C = DecCfg<kHd>;
+    using M = Mma16<T>;
+    constexpr int kSteps = kHd / 16, kBlocks = kHd / 64;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
+    __shared__ float s_m[C::kWarps][16], s_l[C::kWarps][16];
+    __shared__ PagedCut cut;
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* s_o = reinterpret_cast<float*>(smem + C::kStages * 2 * C::kTile);  // [warp][16][kJoinDims]
+    const PagedLaunch& A = P.a;
+    const PagedKv& kv = A.c;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int G = kv.nh / kv.nkv, tt = A.tl.tt;
+    if (tid == 0) {
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], C::kWarps);
+        }
+        fence_mbar_init();
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);  // synchronises the block
+    PagedWalk w;
+    w.begin(cut);
+
+    if (warp == C::kWarps) {
+        // ---- producer: the whole warp, a box per lane
+        int it = 0, issued = 0;
+        while (w.next(kv, A.max_q, tt, C::kKeys)) {
+            const int page_shift = kv.page_shift, bs = P.box_shift;
+            const int last = min((w.rt + 1) * tt, w.s.q_len);
+            const int keys = w.s.kv_len - w.s.q_len + last;  // positions the item's rows attend
+            const int32_t* table = kv.table + w.b * kv.max_pages;
+            int have = -1, id = 0;  // pages have .. have + 31 of the sequence, one per lane
+            bool stop = false;
+            for (int t = w.t0; t < w.t1; ++t, ++it) {
+                const int st = it % C::kStages;
+                const int k0 = t * C::kKeys, n = max(0, min(C::kKeys, keys - k0));
+                const int boxes = (n + (1 << bs) - 1) >> bs;
+                const int p0 = k0 >> page_shift, p1 = n > 0 ? (k0 + n - 1) >> page_shift : p0;
+                if (n > 0 && (have < 0 || p0 < have || p1 >= have + 32)) {
+                    have = p0;
+                    id = -2;
+                    if (p0 + lane <= (keys - 1) >> page_shift) {
+                        id = table[p0 + lane];
+                        if (id < 0 || id >= kv.num_pages) {
+                            record_error(kv.status, DEV_BAD_INDEX);
+                            id = static_cast<int>(kv.num_pages);  // outside the map: zeros are loaded
+                        }
+                    }
+                }
+                if (it >= C::kStages && !mbar_wait(&empty[st], ((it / C::kStages) - 1) & 1, kv.status)) stop = true;
+                if (__any_sync(0xffffffffu, stop)) {
+                    stop = true;
+                    break;
+                }
+                const uint32_t box_bytes = 128u << bs;
+                if (lane == 0)
+                    mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(boxes) * kBlocks * 2u * box_bytes);
+                __syncwarp();
+                ++issued;
+                unsigned char* kd = smem + st * 2 * C::kTile;
+                for (int i0 = 0; i0 < boxes * kBlocks * 2; i0 += 32) {
+                    const int i = i0 + lane;
+                    const int box = i / (kBlocks * 2), part = i % (kBlocks * 2);  // part: K blocks, then V blocks
+                    const int key = k0 + (box << bs);
+                    const int page = __shfl_sync(0xffffffffu, id, ((key >> page_shift) - have) & 31);
+                    if (i < boxes * kBlocks * 2) {
+                        const int blk = part % kBlocks;
+                        const bool v = part >= kBlocks;
+                        tma_page(kd + (v ? C::kTile : 0) + blk * C::kKeys * 128 + (box << bs) * 128, v ? &P.vmap : &P.kmap,
+                                 blk * 64, key & ((1 << page_shift) - 1), w.h, page, &full[st]);
+                    }
+                }
+            }
+            if (stop) break;
+        }
+        // copies in flight end before the block does
+        if (lane == 0)
+            for (int i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
+                mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, nullptr, kDrainNs);
+        return;
+    }
+
+    // ---- consumers
+    const int g4 = lane >> 2, c4 = lane & 3;
+    const uint32_t ring = smem_u32(smem);
+    // ldmatrix rows: K matrices (keys 0-7, dims 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15);
+    // V matrices (keys 0-7, dims 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
+    const int kkey = 16 * warp + (lane >> 4) * 8 + (lane & 7), kchunk = (lane >> 3) & 1;
+    const int vkey = 16 * warp + ((lane >> 3) & 1) * 8 + (lane & 7), vchunk = lane >> 4;
+    PagedJoin join{0, 0, 0, 0, 0};
+    int it = 0;
+    bool late = false;
+    while (w.next(kv, A.max_q, tt, C::kKeys)) {
+        // this thread's two rows
+        int gr[2], tok[2];
+        uint32_t qa[kSteps][4];
+        int pos[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            tok[r] = paged_row_token(g4 + 8 * r, 16, G, w.rt, tt, w.s.q_len, &gr[r]);
+            pos[r] = tok[r] >= 0 ? w.s.kv_len - w.s.q_len + tok[r] : -1;
+            const T* src = static_cast<const T*>(A.q) + (w.s.row0 + (tok[r] < 0 ? 0 : tok[r])) * A.q_stride +
+                           (w.h * G + gr[r]) * kHd + 2 * c4;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    qa[k][r + 2 * x] =
+                        tok[r] >= 0 ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 * x) : 0u;
+        }
+        const int first_pos = w.s.kv_len - w.s.q_len + w.rt * tt;  // the least position of the item's rows
+        const int keys = w.s.kv_len - w.s.q_len + min((w.rt + 1) * tt, w.s.q_len);
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        float o[kHd / 8][4];
+#pragma unroll
+        for (int i = 0; i < kHd / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+        for (int t = w.t0; t < w.t1; ++t, ++it) {
+            const int st = it % C::kStages;
+            // after a wait that ran out (recorded in the status) nothing is waited for any more
+            if (!late && !mbar_wait(&full[st], (it / C::kStages) & 1, kv.status)) late = true;
+            const uint32_t kb = ring + st * 2 * C::kTile, vb = kb + C::kTile;
+            float s[2][4] = {};
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t b[4];
+                const int ch = 2 * (k & 3) + kchunk;
+                ldsm4(kb + (k >> 2) * (C::kKeys * 128) + kkey * 128 + ((ch ^ (kkey & 7)) << 4), b);
+                M::mma(s[0], qa[k], b[0], b[1]);
+                M::mma(s[1], qa[k], b[2], b[3]);
+            }
+            const int j0 = t * C::kKeys + 16 * warp + 2 * c4;  // this thread's keys: j0 + {0, 1, 8, 9}
+            const bool edge = (t + 1) * C::kKeys > first_pos + 1;
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    float v = s[n][x] * A.o.sl2;
+                    if (edge && j0 + 8 * n + (x & 1) > pos[x >> 1]) v = -INFINITY;
+                    s[n][x] = v;
+                    mx[x >> 1] = fmaxf(mx[x >> 1], v);
+                }
+            float f[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                const float mn = fmaxf(m[r], mx[r]);
+                f[r] = mn == -INFINITY ? 1.0f : ex2(m[r] - mn);
+                m[r] = mn;
+            }
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float ms = m[r] == -INFINITY ? 0.0f : m[r];
+                l[r] *= f[r];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float p0 = ex2(s[n][2 * r] - ms), p1 = ex2(s[n][2 * r + 1] - ms);
+                    l[r] += p0 + p1;
+                    const uint32_t h = M::pack(p0, p1);
+                    const float2 u = M::unpack(h);
+                    ph[r + 2 * n] = h;
+                    pl[r + 2 * n] = M::pack(p0 - u.x, p1 - u.y);
+                }
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < kHd / 8; ++i) {
+                    o[i][0] *= f[0];
+                    o[i][1] *= f[0];
+                    o[i][2] *= f[1];
+                    o[i][3] *= f[1];
+                }
+            }
+            // positions behind the item's last key hold whatever the page or the ring held: no 0 * NaN
+            uint32_t va = 0xFFFFFFFFu, vz = 0xFFFFFFFFu;
+            const bool tail = (t + 1) * C::kKeys > keys;
+            if (tail) {
+                va = (j0 < keys ? 0xFFFFu : 0u) | (j0 + 1 < keys ? 0xFFFF0000u : 0u);
+                vz = (j0 + 8 < keys ? 0xFFFFu : 0u) | (j0 + 9 < keys ? 0xFFFF0000u : 0u);
+            }
+#pragma unroll
+            for (int d = 0; d < kHd / 16; ++d) {
+                uint32_t b[4];
+                const int ch = 2 * (d & 3) + vchunk;
+                ldsm4t(vb + (d >> 2) * (C::kKeys * 128) + vkey * 128 + ((ch ^ (vkey & 7)) << 4), b);
+                if (tail) {
+                    b[0] &= va;
+                    b[1] &= vz;
+                    b[2] &= va;
+                    b[3] &= vz;
+                }
+                M::mma(o[2 * d], ph, b[0], b[1]);
+                M::mma(o[2 * d + 1], ph, b[2], b[3]);
+                M::mma(o[2 * d], pl, b[0], b[1]);
+                M::mma(o[2 * d + 1], pl, b[2], b[3]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+        // ---- the item's end: join the four warps
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (c4 == 0) {
+                s_m[warp][g4 + 8 * r] = m[r];
+                s_l[warp][g4 + 8 * r] = l[r];
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        float wf[2];  // this warp's weights
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float mm = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < C::kWarps; ++i) mm = fmaxf(mm, s_m[i][g4 + 8 * r]);
+            wf[r] = m[r] == -INFINITY ? 0.0f : ex2(m[r] - mm);
+        }
+        // the rows as they are written: thread (row tid / 8, columns 4 (tid % 8) .. + 3)
+        const int row = tid >> 3, cq = (tid & 7) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C::kWarps; ++i) mm = fmaxf(mm, s_m[i][row]);
+#pragma unroll
+        for (int i = 0; i < C::kWarps; ++i) ll += s_m[i][row] == -INFINITY ? 0.0f : s_l[i][row] * ex2(s_m[i][row] - mm);
+        int og;
+        const int ot = paged_row_token(row, 16, G, w.rt, tt, w.s.q_len, &og);
+        const int64_t orow = (w.s.row0 + (ot < 0 ? 0 : ot)) * kv.nh + w.h * G + og;
+        const bool whole = w.whole();
+        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + w.slot();
+        const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+        for (int d0 = 0; d0 < kHd; d0 += C::kJoinDims) {
+#pragma unroll
+            for (int i = 0; i < C::kJoinDims / 8; ++i)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int oi = d0 / 8 + i;
+                    *reinterpret_cast<float2*>(s_o + (warp * 16 + g4 + 8 * r) * C::kJoinDims + 8 * i + 2 * c4) =
+                        make_float2(o[oi][2 * r] * wf[r], o[oi][2 * r + 1] * wf[r]);
+                }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < C::kWarps; ++i) {
+                const float4 u = *reinterpret_cast<const float4*>(s_o + (i * 16 + row) * C::kJoinDims + cq);
+                v.x += u.x;
+                v.y += u.y;
+                v.z += u.z;
+                v.w += u.w;
+            }
+            if (whole) {
+                if (ot >= 0)
+                    *reinterpret_cast<uint2*>(static_cast<T*>(A.o.out) + orow * kHd + d0 + cq) =
+                        make_uint2(M::pack(v.x * inv, v.y * inv), M::pack(v.z * inv, v.w * inv));
+            } else {
+                *reinterpret_cast<float4*>(A.sc.o + (slot * 16 + row) * kHd + d0 + cq) = v;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
+        if ((tid & 7) == 0) {
+            if (whole) {
+                if (A.o.lse && ot >= 0) A.o.lse[orow] = ll > 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+            } else {
+                *reinterpret_cast<float2*>(A.sc.ml + (slot * 16 + row) * 2) = make_float2(mm, ll);
+            }
+        }
+        if (!whole && w.t0 == 0)
+            join = PagedJoin{w.s.row0, w.s.q_len, w.h, w.rt,
+                             static_cast<int>((w.at - (w.t1 - w.t0) + w.tiles - 1) / cut.per) - static_cast<int>(blockIdx.x) + 1};
+    }
+    if (tid == 0) A.sc.join[blockIdx.x] = join;
+}
+
+// ---------------------------------------------------------------- joining the pieces of cut items
+// CTA (w, part): 16 rows of the item that CTA w began and others finished: maxima first, then the
+// outputs weighted by 2^(m_i - m), in the pieces' order.
+constexpr int kCombineRows = 16;
+template <typename Out, int kHd>
+__global__ void __launch_bounds__(256) k_paged_combine(const PagedLaunch A) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const PagedJoin j = A.sc.join[blockIdx.x];
+    if (j.pieces == 0) return;
+    const int G = A.c.nh / A.c.nkv, rows = A.tl.rows;
+    constexpr int kCols = kHd / 16;  // columns of a thread
+    const int row = blockIdx.y * kCombineRows + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * kCols;
+    int g;
+    const int tok = paged_row_token(row, A.tl.sub, G, j.rt, A.tl.tt, j.q_len, &g);
+    if (tok < 0) return;
+    // piece i: slot 1 of CTA w for the first, slot 0 of CTA w + i for the others
+    auto slot = [&](int i) { return static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < j.pieces; ++i) m = fmaxf(m, A.sc.ml[(slot(i) * rows + row) * 2]);
+    float o[kCols] = {};
+    if (m > -INFINITY)
+        for (int i = 0; i < j.pieces; ++i) {
+            const float2 ml = *reinterpret_cast<const float2*>(A.sc.ml + (slot(i) * rows + row) * 2);
+            const float f = ex2(ml.x - m);
+            l += f * ml.y;
+            const float* src = A.sc.o + (slot(i) * rows + row) * kHd + c0;
+#pragma unroll
+            for (int c = 0; c < kCols; c += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src + c);
+                o[c] += f * v.x;
+                o[c + 1] += f * v.y;
+                o[c + 2] += f * v.z;
+                o[c + 3] += f * v.w;
+            }
+        }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int64_t orow = (j.row0 + tok) * A.c.nh + j.h * G + g;
+    Out* dst = static_cast<Out*>(A.o.out) + orow * kHd + c0;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+        const float v = o[c] * inv;
+        if constexpr (sizeof(Out) == 4) dst[c] = v;
+        else if constexpr (std::is_same<Out, __half>::value) dst[c] = __float2half_rn(v);
+        else dst[c] = __float2bfloat16_rn(v);
+    }
+    if (A.o.lse && (threadIdx.x & 15) == 0) A.o.lse[orow] = l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+}
+
+template <typename Out>
+static cudaError_t launch_combine_t(const PagedLaunch& a, int hd, int ctas, cudaStream_t s) {
+    const dim3 grid(static_cast<unsigned>(ctas), static_cast<unsigned>(a.tl.rows / kCombineRows));
+    return hd == 128 ? launch_pdl(k_paged_combine<Out, 128>, grid, dim3(256), 0, s, a)
+                     : launch_pdl(k_paged_combine<Out, 64>, grid, dim3(256), 0, s, a);
+}
+cudaError_t launch_paged_combine(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s) {
+    return out_dtype == SC_F16    ? launch_combine_t<__half>(a, hd, ctas, s)
+           : out_dtype == SC_BF16 ? launch_combine_t<__nv_bfloat16>(a, hd, ctas, s)
+                                  : launch_combine_t<float>(a, hd, ctas, s);
+}
+
+template <typename T, int kHd>
+static cudaError_t launch_decode_t(const DecodeParams& p, int ctas, cudaStream_t s) {
+    using C = DecCfg<kHd>;
+    static std::atomic<uint64_t> flags{0};
+    cudaError_t e = paged_allow_smem(k_paged_decode<T, kHd>, flags, C::kSmem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_paged_decode<T, kHd>, dim3(static_cast<unsigned>(ctas)), dim3(C::kThreads), C::kSmem, s, p);
+}
+
+cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s) {
+    DecodeParams p;
+    p.a = a;
+    p.box_shift = a.c.page_shift < 6 ? a.c.page_shift : 6;
+    cudaError_t e = paged_tensor_map(&p.kmap, a.c, a.c.k, dtype, hd, 1 << p.box_shift);
+    if (e == cudaSuccess) e = paged_tensor_map(&p.vmap, a.c, a.c.v, dtype, hd, 1 << p.box_shift);
+    if (e != cudaSuccess) return e;
+    if (dtype == SC_F16)
+        return hd == 128 ? launch_decode_t<__half, 128>(p, ctas, s) : launch_decode_t<__half, 64>(p, ctas, s);
+    return hd == 128 ? launch_decode_t<__nv_bfloat16, 128>(p, ctas, s) : launch_decode_t<__nv_bfloat16, 64>(p, ctas, s);
+}
+
+}  // namespace sc
