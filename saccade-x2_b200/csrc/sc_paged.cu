@@ -233,21 +233,36 @@ static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
     return fn;
 }
 
-cudaError_t paged_tensor_map(CUtensorMap* map, const PagedKv& c, const void* pages, int dtype, int hd, int box_rows) {
+static cudaError_t encode_map(CUtensorMap* map, const void* base, int dtype, const cuuint64_t (&dims)[4],
+                              const cuuint64_t (&strides)[3], const cuuint32_t (&box)[4], CUtensorMapL2promotion l2) {
     PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
     if (!encode) return cudaErrorNotSupported;
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, dtype == SC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                              const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, l2, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t paged_tensor_map(CUtensorMap* map, const PagedKv& c, const void* pages, int dtype, int hd, int box_rows) {
     const cuuint64_t page = 1ull << c.page_shift;
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), page, static_cast<cuuint64_t>(c.nkv),
                                 static_cast<cuuint64_t>(c.num_pages)};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(hd) * 2, page * hd * 2,
                                    static_cast<cuuint64_t>(c.page_stride) * 2};
     const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
-    const cuuint32_t es[4] = {1, 1, 1, 1};
-    const CUresult r = encode(map, dtype == SC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                              const_cast<void*>(pages), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+    return encode_map(map, pages, dtype, dims, strides, box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+cudaError_t paged_query_map(CUtensorMap* map, const PagedLaunch& a, int dtype, int hd, int box_tokens) {
+    const int G = a.c.nh / a.c.nkv;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(G),
+                                static_cast<cuuint64_t>(a.c.nkv), static_cast<cuuint64_t>(a.c.tokens)};
+    // a single row's stride is never used, but must be a legal one
+    const cuuint64_t row = a.c.tokens > 1 ? static_cast<cuuint64_t>(a.q_stride) * 2 : static_cast<cuuint64_t>(a.c.nh) * hd * 2;
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(hd) * 2, static_cast<cuuint64_t>(G) * hd * 2, row};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(G), 1, static_cast<cuuint32_t>(box_tokens)};
+    return encode_map(map, a.q, dtype, dims, strides, box, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 static int sm_count() {
@@ -262,17 +277,15 @@ static int sm_count() {
 
 // The kernel of a call and its work division.
 struct PagedPlan {
-    bool decode;           // the 16-row kernel
+    enum Kind { kPlain, kDecode, kChunk } kind;
     int ctas;
     PagedTiling tl;
 };
 static PagedPlan paged_plan(int dtype, int nh, int nkv, int64_t max_q) {
-    PagedPlan p{};
     const int G = nh / nkv;
-    p.decode = dtype != SC_F32 && max_q * G <= 16;
-    p.ctas = 2 * sm_count();
-    p.tl = PagedTiling{16, 16, G <= 16 ? 16 / G : 1, 64};
-    return p;
+    if (dtype == SC_F32) return {PagedPlan::kPlain, 0, {}};
+    if (max_q * G <= 16) return {PagedPlan::kDecode, 2 * sm_count(), {16, 16, 16 / G, 64}};
+    return {PagedPlan::kChunk, sm_count(), {256, 128, 2 * (128 / G), 128}};
 }
 
 static int64_t elem_size(int dtype) { return dtype == SC_F32 ? 4 : 2; }
@@ -383,7 +396,7 @@ size_t sc_qwen2_paged_attention_scratch(int64_t tokens, int64_t num_seqs, int nu
     (void)tokens, (void)num_seqs;
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || max_q_len <= 0) return 0;
     const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, max_q_len);
-    return p.decode ? paged_scratch_bytes(p.ctas, p.tl.rows, head_dim) : 0;
+    return p.kind == PagedPlan::kPlain ? 0 : paged_scratch_bytes(p.ctas, p.tl.rows, head_dim);
 }
 
 sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
@@ -404,7 +417,7 @@ sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* 
     if (out_dtype != cache_dtype && !(cache_dtype == SC_F32 && out_dtype == SC_F16))
         return paged_bad(who, "out is of the cache's type, or f16 from an f32 cache");
     if (max_q_len <= 0 || max_kv_len <= 0) return paged_bad(who, "max_q_len and max_kv_len must be positive");
-    if (!(scale == scale) || scale - scale != 0.0f) return paged_bad(who, "scale must be finite");
+    if (!(scale > 0.0f) || scale - scale != 0.0f) return paged_bad(who, "scale must be positive and finite");
     const int64_t cs = elem_size(cache_dtype);
     if (tokens > 1 && q_stride < static_cast<int64_t>(num_heads) * head_dim) return paged_bad(who, "rows of q overlap");
     if (!aligned16(q) || (tokens > 1 && q_stride * cs % 16) || !aligned16(k_pages) || !aligned16(v_pages) ||
@@ -417,11 +430,12 @@ sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* 
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, max_q_len);
-    if (p.decode) {
+    if (p.kind != PagedPlan::kPlain) {
         if (!scratch || !aligned16(scratch)) return paged_bad(who, "scratch must be 16-byte aligned");
         const PagedLaunch a{c, q, q_stride, max_q_len, {out, lse, scale * 1.4426950408889634f}, p.tl,
                             paged_scratch(scratch, p.ctas, p.tl.rows, head_dim)};
-        cudaError_t e = launch_paged_decode(a, cache_dtype, head_dim, p.ctas, s);
+        cudaError_t e = p.kind == PagedPlan::kDecode ? launch_paged_decode(a, cache_dtype, head_dim, p.ctas, s)
+                                                     : launch_paged_chunk(a, cache_dtype, head_dim, p.ctas, s);
         if (e == cudaSuccess) e = launch_paged_combine(a, out_dtype, head_dim, p.ctas, s);
         return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
     }

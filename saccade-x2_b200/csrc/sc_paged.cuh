@@ -251,6 +251,43 @@ __device__ __forceinline__ int paged_row_token(int r, int sub, int group, int rt
     return tok < per && t < q_len ? t : -1;
 }
 
+// Two f32 as two 16-bit values of the cache's type, and back.
+template <typename T>
+struct Pack16;
+template <>
+struct Pack16<__half> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+};
+template <>
+struct Pack16<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void tma_page(void* smem_dst, const CUtensorMap* map, int col, int row, int head, int page,
+                                         uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
 struct PagedLaunch {
     PagedKv c;
     const void* q;
@@ -262,7 +299,9 @@ struct PagedLaunch {
 };
 
 // The pages as a tensor {head_dim, page, KV heads, pages} with boxes of 64 elements x box_rows positions, each
-// box landing as rows of 128 bytes in the 128-byte swizzle (16-bit caches).
+// box landing as rows of 128 bytes in the 128-byte swizzle (16-bit caches); the queries as {head_dim, query
+// heads of a KV head, KV heads, tokens} with boxes of 64 elements x the group x box_tokens.
+cudaError_t paged_query_map(CUtensorMap* map, const PagedLaunch& a, int dtype, int hd, int box_tokens);
 cudaError_t paged_tensor_map(CUtensorMap* map, const PagedKv& c, const void* pages, int dtype, int hd, int box_rows);
 
 // Raises a kernel's dynamic shared-memory limit once per device.
@@ -279,6 +318,7 @@ cudaError_t paged_allow_smem(Kern kern, std::atomic<uint64_t>& flags, int bytes)
 }
 
 cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
+cudaError_t launch_paged_chunk(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
 cudaError_t launch_paged_combine(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);
 
 }  // namespace sc

@@ -32,49 +32,18 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
 }
 
 template <typename T>
-struct Mma16;
+__device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
-struct Mma16<__half> {
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        mma_16816(d, a, b0, b1);
-    }
-    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-};
-template <>
-struct Mma16<__nv_bfloat16> {
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-            "{%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    static __device__ __forceinline__ float2 unpack(uint32_t v) {
-        return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
-    }
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+__device__ __forceinline__ void mma_16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_16816(d, a, b0, b1);
 }
-
-__device__ __forceinline__ void tma_page(void* smem_dst, const CUtensorMap* map, int col, int row, int head, int page,
-                                         uint64_t* bar) {
+template <>
+__device__ __forceinline__ void mma_16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];" ::"r"(smem_u32(smem_dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
-        : "memory");
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 template <int kHd>
@@ -97,7 +66,7 @@ struct alignas(64) DecodeParams {
 template <typename T, int kHd>
 __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const __grid_constant__ DecodeParams P) {
     using C = DecCfg<kHd>;
-    using M = Mma16<T>;
+    using M = Pack16<T>;
     constexpr int kSteps = kHd / 16, kBlocks = kHd / 64;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
@@ -228,8 +197,8 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                 uint32_t b[4];
                 const int ch = 2 * (k & 3) + kchunk;
                 ldsm4(kb + (k >> 2) * (C::kKeys * 128) + kkey * 128 + ((ch ^ (kkey & 7)) << 4), b);
-                M::mma(s[0], qa[k], b[0], b[1]);
-                M::mma(s[1], qa[k], b[2], b[3]);
+                mma_16<T>(s[0], qa[k], b[0], b[1]);
+                mma_16<T>(s[1], qa[k], b[2], b[3]);
             }
             const int j0 = t * C::kKeys + 16 * warp + 2 * c4;  // this thread's keys: j0 + {0, 1, 8, 9}
             const bool edge = (t + 1) * C::kKeys > first_pos + 1;
@@ -294,10 +263,10 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                     b[2] &= va;
                     b[3] &= vz;
                 }
-                M::mma(o[2 * d], ph, b[0], b[1]);
-                M::mma(o[2 * d + 1], ph, b[2], b[3]);
-                M::mma(o[2 * d], pl, b[0], b[1]);
-                M::mma(o[2 * d + 1], pl, b[2], b[3]);
+                mma_16<T>(o[2 * d], ph, b[0], b[1]);
+                mma_16<T>(o[2 * d + 1], ph, b[2], b[3]);
+                mma_16<T>(o[2 * d], pl, b[0], b[1]);
+                mma_16<T>(o[2 * d + 1], pl, b[2], b[3]);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
