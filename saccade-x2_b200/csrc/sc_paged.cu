@@ -144,71 +144,6 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArg
     }
 }
 
-// ---------------------------------------------------------------- attention, the plain kernel
-// One warp per (token, query head): keys one after the other with a running maximum and sum, each
-// lane holding hd / 32 elements of q and o.
-template <typename T, typename Out, int kHd>
-__global__ void __launch_bounds__(256) k_paged_attn_plain(const T* __restrict__ q, int64_t q_stride, PagedKv c,
-                                                          int64_t max_q, float scale, Out* __restrict__ out,
-                                                          float* __restrict__ lse) {
-    constexpr int kE = kHd / 32;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t item = blockIdx.x * 8ll + (threadIdx.x >> 5);
-    const int64_t t = item / c.nh;
-    const int h = static_cast<int>(item % c.nh);
-    if (t >= c.tokens) return;
-    int seq = 0;
-    for (int b0 = 0; b0 < c.num_seqs; b0 += 32) {
-        const bool before = b0 + lane < c.num_seqs && c.cu_q[b0 + lane + 1] <= t;
-        seq += __popc(__ballot_sync(0xffffffffu, before));
-    }
-    if (seq >= c.num_seqs || t < c.cu_q[seq]) return;
-    const PagedSeq s = paged_seq(c, seq, max_q);
-    if (s.q_len == 0) return;
-    const int pos = s.kv_len - s.q_len + static_cast<int>(t - s.row0);
-    float qf[kE], o[kE] = {};
-#pragma unroll
-    for (int e = 0; e < kE; ++e) qf[e] = to_f32(q[t * q_stride + h * kHd + lane + 32 * e]);
-    float m = -INFINITY, l = 0.0f;
-    const int hk = h / (c.nh / c.nkv);
-    for (int j = 0; j <= pos; ++j) {
-        const int64_t page = c.table[seq * c.max_pages + (j >> c.page_shift)];
-        if (page < 0 || page >= c.num_pages) {
-            record_error(c.status, DEV_BAD_INDEX);
-            continue;
-        }
-        const int64_t at = page * c.page_stride +
-                           ((static_cast<int64_t>(hk) << c.page_shift) + (j & ((1 << c.page_shift) - 1))) * kHd + lane;
-        float d = 0.0f;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) d += qf[e] * to_f32(static_cast<const T*>(c.k)[at + 32 * e]);
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
-        d *= scale;
-        const float mn = fmaxf(m, d), f = expf(m - mn), p = expf(d - mn);
-        l = l * f + p;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) o[e] = o[e] * f + p * to_f32(static_cast<const T*>(c.v)[at + 32 * e]);
-        m = mn;
-    }
-#pragma unroll
-    for (int e = 0; e < kE; ++e)
-        out[(t * c.nh + h) * kHd + lane + 32 * e] = from_f32<Out>(l > 0.0f ? o[e] / l : 0.0f);
-    if (lse && lane == 0) lse[t * c.nh + h] = l > 0.0f ? m + logf(l) : -INFINITY;
-}
-
-template <typename T, typename Out>
-static cudaError_t launch_plain(const void* q, int64_t q_stride, const PagedKv& c, int hd, int64_t max_q, float scale,
-                                void* out, float* lse, cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>((c.tokens * c.nh + 7) / 8));
-    return hd == 128 ? launch_pdl(k_paged_attn_plain<T, Out, 128>, grid, dim3(256), 0, s, static_cast<const T*>(q),
-                                  q_stride, c, max_q, scale, static_cast<Out*>(out), lse)
-                     : launch_pdl(k_paged_attn_plain<T, Out, 64>, grid, dim3(256), 0, s, static_cast<const T*>(q),
-                                  q_stride, c, max_q, scale, static_cast<Out*>(out), lse);
-}
-
 template <typename In, typename Cache>
 static cudaError_t launch_append(const AppendArgs& a, int hd, cudaStream_t s) {
     const int heads_at_once = kAppendThreads / (hd / 16), heads = a.c.nh + 2 * a.c.nkv;
@@ -277,13 +212,16 @@ static int sm_count() {
 
 // The kernel of a call and its work division.
 struct PagedPlan {
-    enum Kind { kPlain, kDecode, kChunk } kind;
+    enum Kind { kF32, kDecode, kChunk } kind;
     int ctas;
     PagedTiling tl;
 };
-static PagedPlan paged_plan(int dtype, int nh, int nkv, int64_t max_q) {
+static PagedPlan paged_plan(int dtype, int nh, int nkv, int hd, int64_t max_q) {
     const int G = nh / nkv;
-    if (dtype == SC_F32) return {PagedPlan::kPlain, 0, {}};
+    if (dtype == SC_F32) {
+        if (max_q * G <= 16) return {PagedPlan::kF32, 2 * sm_count(), {16, 16, 16 / G, 64}};
+        return {PagedPlan::kF32, hd == 64 ? 2 * sm_count() : sm_count(), {64, 64, 64 / G, 64}};
+    }
     if (max_q * G <= 16) return {PagedPlan::kDecode, 2 * sm_count(), {16, 16, 16 / G, 64}};
     return {PagedPlan::kChunk, sm_count(), {256, 128, 2 * (128 / G), 128}};
 }
@@ -394,9 +332,11 @@ sc_status sc_qwen2_paged_append(const void* q, const void* k, const void* v, int
 size_t sc_qwen2_paged_attention_scratch(int64_t tokens, int64_t num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                         int64_t max_q_len, int cache_dtype) {
     (void)tokens, (void)num_seqs;
-    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || max_q_len <= 0) return 0;
-    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, max_q_len);
-    return p.kind == PagedPlan::kPlain ? 0 : paged_scratch_bytes(p.ctas, p.tl.rows, head_dim);
+    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_heads / num_kv_heads > kPagedMaxGroup ||
+        max_q_len <= 0)
+        return 0;
+    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, head_dim, max_q_len);
+    return paged_scratch_bytes(p.ctas, p.tl.rows, head_dim);
 }
 
 sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
@@ -429,22 +369,14 @@ sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* 
         return SC_ENOMEM;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, max_q_len);
-    if (p.kind != PagedPlan::kPlain) {
-        if (!scratch || !aligned16(scratch)) return paged_bad(who, "scratch must be 16-byte aligned");
-        const PagedLaunch a{c, q, q_stride, max_q_len, {out, lse, scale * 1.4426950408889634f}, p.tl,
-                            paged_scratch(scratch, p.ctas, p.tl.rows, head_dim)};
-        cudaError_t e = p.kind == PagedPlan::kDecode ? launch_paged_decode(a, cache_dtype, head_dim, p.ctas, s)
-                                                     : launch_paged_chunk(a, cache_dtype, head_dim, p.ctas, s);
-        if (e == cudaSuccess) e = launch_paged_combine(a, out_dtype, head_dim, p.ctas, s);
-        return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
-    }
-    const cudaError_t e =
-        cache_dtype == SC_F16 ? launch_plain<__half, __half>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s)
-        : cache_dtype == SC_BF16
-            ? launch_plain<__nv_bfloat16, __nv_bfloat16>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s)
-        : out_dtype == SC_F16 ? launch_plain<float, __half>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s)
-                              : launch_plain<float, float>(q, q_stride, c, head_dim, max_q_len, scale, out, lse, s);
+    if (!scratch || !aligned16(scratch)) return paged_bad(who, "scratch must be 16-byte aligned");
+    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, head_dim, max_q_len);
+    const PagedLaunch a{c, q, q_stride, max_q_len, {out, lse, scale * 1.4426950408889634f}, p.tl,
+                        paged_scratch(scratch, p.ctas, p.tl.rows, head_dim)};
+    cudaError_t e = p.kind == PagedPlan::kF32      ? launch_paged_f32(a, out_dtype, head_dim, p.ctas, s)
+                    : p.kind == PagedPlan::kDecode ? launch_paged_decode(a, cache_dtype, head_dim, p.ctas, s)
+                                                   : launch_paged_chunk(a, cache_dtype, head_dim, p.ctas, s);
+    if (e == cudaSuccess) e = launch_paged_combine(a, out_dtype, head_dim, p.ctas, s);
     return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
 }
 

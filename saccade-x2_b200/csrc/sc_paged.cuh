@@ -319,6 +319,7 @@ cudaError_t paged_allow_smem(Kern kern, std::atomic<uint64_t>& flags, int bytes)
 
 cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
 cudaError_t launch_paged_chunk(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
+cudaError_t launch_paged_f32(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);
 cudaError_t launch_paged_combine(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);
 
 }  // namespace sc

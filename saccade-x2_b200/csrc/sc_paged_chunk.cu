@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                 for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sr[i]));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
                 if (__any_sync(0xffffffffu, top > m + kMove)) {
-                    const float mn = top > m ? fmaxf(m, top - kShift) : m;
+                    const float mn = top > m + kMove ? top - kShift : m;  // each row by itself
                     if (j > 0) {
                         const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
                         l *= f;
