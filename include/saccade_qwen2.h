@@ -147,6 +147,10 @@ SC_API sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const
                                           float scale, void* out, int out_dtype, float* lse, void* scratch,
                                           size_t scratch_bytes, uint32_t* status, void* stream);
 
+/* Scratch bytes sc_qwen2_process_logits needs for best / best_value (no initial contents; one call uses
+ * it at a time); without both it needs none. */
+SC_API size_t sc_qwen2_process_logits_scratch(int64_t rows, int64_t vocab);
+
 /* Logits [rows][vocab] of dtype (SC_F32, SC_F16, SC_BF16), rows `stride` apart, of the tokens vocab_begin ..
  * vocab_begin + vocab (a tensor-parallel rank's slice; every id below is of the whole vocabulary) ->
  * out (out_stride apart; may be logits itself).  Per row and token v, in f32 and rounded once:
@@ -162,7 +166,8 @@ SC_API sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const
  * best (nullable int64 [rows]) and best_value (nullable, dtype [rows]): the id and value of the largest
  * output, the first of equals, NaN above all as torch.argmax has it.  A length, mask row or number of
  * bias entries out of range records SC_EDEVICE in *status (nullable) and is cut to what there is (a
- * mask row: no mask).  history_stride <= 524287 and vocab <= 2^30, SC_EINVAL otherwise. */
+ * mask row: no mask).  history_stride <= 524287, rows <= 2^20 and vocab_begin + vocab <= 2^30, SC_EINVAL
+ * otherwise. */
 SC_API sc_status sc_qwen2_process_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
                                          int64_t vocab_begin, const int32_t* history, int64_t history_stride,
                                          const int32_t* prompt_len, const int32_t* hist_len, const float* repetition,
@@ -170,7 +175,8 @@ SC_API sc_status sc_qwen2_process_logits(const void* logits, int dtype, int64_t 
                                          const int32_t* bias_ids, const float* bias_vals, int64_t num_bias,
                                          const int32_t* mask, int64_t mask_words, int64_t mask_rows,
                                          const int32_t* mask_row, void* out, int64_t out_stride, int64_t* best,
-                                         void* best_value, uint32_t* status, void* stream);
+                                         void* best_value, void* scratch, size_t scratch_bytes, uint32_t* status,
+                                         void* stream);
 
 SC_API sc_status sc_qwen2_f16_to_f32(const uint16_t* x, int64_t n, float* out, void* stream);
 

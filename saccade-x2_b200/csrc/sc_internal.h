@@ -111,6 +111,8 @@ sc_status cuda_fail(cudaError_t e, const char* what);
 // Dynamic shared memory of the router kernels (the token row, f16): K <= 65536.
 constexpr int kRouterMaxRowBytes = 128 * 1024;
 
+int sm_count();  // multiprocessors of the current device (148 where there is none)
+
 // Kernels this library has launched (host-side count of launch calls, sc_launch_count).
 extern std::atomic<uint64_t> g_launches;
 

@@ -7,15 +7,15 @@
 //   y  = allowed(v) ? x3 : -inf
 // One pass: each logit is read once and written once; the floor is rows * vocab * 2 * size bytes.
 //
-// A row belongs to one thread-block cluster, each CTA of it to a slice of the vocabulary.  The
-// counts n(v) of a slice live in the CTA's shared memory, one word per token: history ids are read
-// once per row (each CTA takes its share of them) and counted by remote shared-memory atomics into
-// the CTA that owns the token, so nothing of vocabulary size ever goes to global memory.  Integer
-// atomics only: the result does not depend on their order.
+// A CTA has a tile of a row's vocabulary.  The counts n(v) of its tokens live in its shared memory, one
+// word per token, so nothing of vocabulary size ever goes to global memory; every CTA of a row goes over
+// the row's whole history (a few KB from L2, tiles x 4 bytes per id) and counts its own tokens with integer
+// atomics, whose order does not matter.  (Thread-block clusters that read the history once and count into each
+// other's shared memory measured slower: 39 us against 21 at 64 x 152064 f32 with 768 ids, two cluster barriers
+// and 31 clusters of 16 at a time.)
 //   word = (bias entry + 1) << 20 | n << 1 | in the prompt
-// Each CTA issues the loads of its first logits before it counts, so that they arrive meanwhile.
-#include <cooperative_groups.h>
-
+// Each CTA issues the loads of its first logits before it counts, so that they arrive meanwhile.  The best of
+// each tile goes to the scratch, and a second small kernel picks each row's.
 #include <atomic>
 #include <string>
 
@@ -25,11 +25,12 @@
 
 namespace sc {
 
-constexpr int kLogitThreads = 512;
-constexpr int kLogitWords = 20480;        // tokens of one CTA's slice at a time (80 KB of words: two CTAs per SM)
+constexpr int kLogitThreads = 256;
+constexpr int kLogitWords = 10240;        // tokens of a tile at most (40 KB of words: four CTAs per SM)
+constexpr int kLogitMinTile = 2048;
 constexpr int kLogitBatch = 6;            // 16-byte loads a thread has in flight
-constexpr int kLogitMaxCluster = 8;
 constexpr int64_t kLogitMaxHistory = (1 << 19) - 1;  // 19 bits of a word count occurrences
+constexpr int64_t kLogitMaxRows = 1 << 20;
 constexpr int kLogitMaxBias = (1 << 12) - 1;         // 12 bits name the bias entry
 
 struct LogitArgs {
@@ -51,8 +52,8 @@ struct LogitArgs {
     int64_t* best;
     void* best_value;
     uint32_t* status;
-    int64_t slice;    // tokens of one CTA and chunk, at most kLogitWords
-    int chunks;       // chunks of cluster * slice tokens
+    int tile, tiles;  // tokens of a tile, tiles of a row
+    uint64_t* keys;   // [rows][tiles], or null
 };
 
 template <typename T>
@@ -84,14 +85,11 @@ __device__ __forceinline__ uint64_t best_key(float v, uint32_t i) {
     return (static_cast<uint64_t>(ord) << 32) | (0xFFFFFFFFu - i);
 }
 
-__device__ __forceinline__ void red_add_cluster(uint32_t addr, uint32_t v) {
-    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void red_or_cluster(uint32_t addr, uint32_t v) {
-    asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 // One logit.  Multiplications and subtractions round one by one.
@@ -107,168 +105,177 @@ __device__ __forceinline__ float process_one(float x, uint32_t word, float rep, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogitThreads, 2) k_process_logits(const LogitArgs a) {
+__global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const LogitArgs a) {
     constexpr int kVec = LogitIo<T>::kVec;
-    extern __shared__ __align__(16) uint32_t words[];  // [slice, rounded up to kVec, + kVec]
+    extern __shared__ __align__(16) uint32_t words[];  // one per token of the tile, from its first vector on
     __shared__ uint64_t s_best[kLogitThreads / 32];
-    __shared__ uint64_t s_all[kLogitMaxCluster];
     pdl_launch_dependents();
-    pdl_wait();
-    const int rank = static_cast<int>(cluster_rank());
-    const int cn = static_cast<int>(cooperative_groups::this_cluster().num_blocks());
-    const int64_t row = blockIdx.x / cn;
+    const int64_t row = blockIdx.x / a.tiles;
     const int tid = threadIdx.x;
-    const T* x = static_cast<const T*>(a.x) + row * a.stride;
-    T* y = static_cast<T*>(a.out) + row * a.out_stride;
-
-    // the row's parameters
-    const float rep = a.rep ? a.rep[row] : 1.0f, pres = a.pres ? a.pres[row] : 0.0f, freq = a.freq ? a.freq[row] : 0.0f;
-    int64_t hist = 0, prompt = 0;
-    if (a.history) {
-        hist = a.hist_len[row];
-        prompt = a.prompt_len ? a.prompt_len[row] : 0;
-        if (hist < 0 || hist > a.history_stride || prompt < 0 || prompt > hist) {
-            if (tid == 0 && rank == 0) record_error(a.status, DEV_BAD_INDEX);
-            hist = hist < 0 ? 0 : imin64(hist, a.history_stride);
-            prompt = prompt < 0 ? 0 : imin64(prompt, hist);
+    // the tile's tokens [t0, t0 + len); vector j covers tokens t0 - lead + j * kVec .. + kVec, so that it starts on a
+    // 16-byte boundary of the row; vectors [full0, full1) lie inside
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x - row * a.tiles) * a.tile;
+    const int len = static_cast<int>(imin64(a.vocab - t0, a.tile));
+    const T* x = static_cast<const T*>(a.x) + row * a.stride + t0;
+    const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    const int nvec = (len + lead + kVec - 1) / kVec;
+    const int full0 = lead ? 1 : 0, full1 = (len + lead) / kVec;
+    const T* xb = x - lead;
+    T* yb = static_cast<T*>(a.out) + row * a.out_stride + t0 - lead;
+    const bool same = (reinterpret_cast<uintptr_t>(yb) & 15u) == 0;
+    auto load = [&](int j) {
+        uint4 r;
+        if (j >= full0 && j < full1) {
+            r = __ldcs(reinterpret_cast<const uint4*>(xb) + j);
+        } else {
+            __align__(16) T v[kVec];
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) {
+                const int e = j * kVec + k;
+                v[k] = e >= lead && e < lead + len ? xb[e] : T(0.0f);
+            }
+            r = *reinterpret_cast<const uint4*>(v);
         }
+        return r;
+    };
+    pdl_wait();
+
+    // the row's parameters and first logits: every load is issued before the first is needed
+    float rep = a.rep ? a.rep[row] : 1.0f, pres = a.pres ? a.pres[row] : 0.0f, freq = a.freq ? a.freq[row] : 0.0f;
+    int hist = a.history ? a.hist_len[row] : 0, prompt = a.history && a.prompt_len ? a.prompt_len[row] : 0;
+    int64_t b0 = a.bias_ptr ? a.bias_ptr[row] : 0, b1 = a.bias_ptr ? a.bias_ptr[row + 1] : 0;
+    int64_t mrow = a.mask ? (a.mask_row ? a.mask_row[row] : row) : -1;
+    uint4 batch[kLogitBatch];
+#pragma unroll
+    for (int i = 0; i < kLogitBatch; ++i) {
+        const int j = tid + i * kLogitThreads;
+        if (j < nvec) batch[i] = load(j);
+    }
+    bool bad = false;
+    if (a.history) {
+        const int width = static_cast<int>(a.history_stride);
+        bad = hist < 0 || hist > width || prompt < 0 || prompt > hist;
+        hist = min(max(hist, 0), width);
+        prompt = min(max(prompt, 0), hist);
         if (rep == 1.0f && pres == 0.0f && freq == 0.0f) hist = prompt = 0;  // counts change nothing
     }
-    int64_t b0 = 0, b1 = 0;
     if (a.bias_ptr) {
-        b0 = a.bias_ptr[row];
-        b1 = a.bias_ptr[row + 1];
-        if (b0 < 0 || b1 < b0 || b1 > a.num_bias || b1 - b0 > kLogitMaxBias) {
-            if (tid == 0 && rank == 0) record_error(a.status, DEV_BAD_INDEX);
-            b0 = b0 < 0 ? 0 : imin64(b0, a.num_bias);
-            b1 = b1 < b0 ? b0 : imin64(imin64(b1, a.num_bias), b0 + kLogitMaxBias);
-        }
+        bad = bad || b0 < 0 || b1 < b0 || b1 > a.num_bias || b1 - b0 > kLogitMaxBias;
+        b0 = b0 < 0 ? 0 : imin64(b0, a.num_bias);
+        b1 = b1 < b0 ? b0 : imin64(imin64(b1, a.num_bias), b0 + kLogitMaxBias);
     }
-    const uint32_t* mask = nullptr;
-    if (a.mask) {
-        int64_t m = a.mask_row ? a.mask_row[row] : row;
-        if (m >= a.mask_rows) {
-            if (tid == 0 && rank == 0) record_error(a.status, DEV_BAD_INDEX);
-            m = -1;
-        }
-        if (m >= 0) mask = a.mask + m * a.mask_words;
+    if (a.mask && mrow >= a.mask_rows) {
+        bad = true;
+        mrow = -1;
     }
-    const bool touched = hist > 0 || b1 > b0;  // the same in every CTA of the cluster
-
-    uint64_t best = 0;
-    for (int c = 0; c < a.chunks; ++c) {
-        // this CTA's tokens [t0, t1) of the slice; vector j covers tokens t0 - lead + j * kVec .. + kVec, so
-        // that it starts on a 16-byte boundary of the row
-        const int64_t t0 = imin64(a.vocab, (static_cast<int64_t>(c) * cn + rank) * a.slice);
-        const int64_t t1 = imin64(a.vocab, t0 + a.slice);
-        const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x + t0) & 15u) / sizeof(T));
-        const bool same = (reinterpret_cast<uintptr_t>(y + t0) & 15u) == lead * sizeof(T);
-        const int nvec = t1 > t0 ? static_cast<int>((t1 - t0 + lead + kVec - 1) / kVec) : 0;
-        auto load = [&](int j) {
-            uint4 r = make_uint4(0, 0, 0, 0);
-            const int64_t e = t0 - lead + static_cast<int64_t>(j) * kVec;
-            if (e >= t0 && e + kVec <= t1) {
-                r = __ldcs(reinterpret_cast<const uint4*>(x + e));
-            } else {  // the slice's first or last vector
-                __align__(16) T v[kVec];
-#pragma unroll
-                for (int k = 0; k < kVec; ++k) v[k] = (e + k >= t0 && e + k < t1) ? x[e + k] : T(0.0f);
-                r = *reinterpret_cast<const uint4*>(v);
-            }
-            return r;
-        };
-        uint4 batch[kLogitBatch];
-#pragma unroll
-        for (int i = 0; i < kLogitBatch; ++i) {
-            const int j = tid + i * kLogitThreads;
-            if (j < nvec) batch[i] = load(j);
+    if (bad && tid == 0) record_error(a.status, DEV_BAD_INDEX);
+    const uint32_t* mask = mrow >= 0 ? a.mask + mrow * a.mask_words : nullptr;
+    const int first = static_cast<int>(t0 + a.begin);  // the tile's first token id
+    const int nb = static_cast<int>(b1 - b0);
+    const bool touched = hist > 0 || nb > 0;
+    if (touched) {
+        for (int i = tid; i < nvec * (kVec / 4); i += kLogitThreads)
+            reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        for (int i = tid; i < nb; i += kLogitThreads) {
+            const int v = a.bias_ids[b0 + i];
+            if (v >= first && v - first < len) atomicMax(&words[v - first + lead], static_cast<uint32_t>(i + 1) << 20);
         }
-        if (touched) {
-            for (int i = tid; i < (nvec * kVec + 3) / 4; i += kLogitThreads)
-                reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
-            __syncthreads();
-            // every CTA goes over all of the row's bias entries (at most 4095) for its own tokens
-            for (int64_t i = b0 + tid; i < b1; i += kLogitThreads) {
-                const int64_t v = a.bias_ids[i] - a.begin;
-                if (v >= t0 && v < t1) atomicMax(&words[v - t0 + lead], static_cast<uint32_t>(i - b0 + 1) << 20);
-            }
-            __syncwarp();
-            cluster_sync();
-            // its share of the history goes to the owners' words
-            const uint32_t base = smem_u32(words);
-            const int64_t c0 = static_cast<int64_t>(c) * cn * a.slice;
-            for (int64_t i = static_cast<int64_t>(rank) * kLogitThreads + tid; i < hist;
-                 i += static_cast<int64_t>(cn) * kLogitThreads) {
-                const int64_t v = a.history[row * a.history_stride + i] - a.begin;
-                if (v < c0 || v >= a.vocab || v - c0 >= cn * a.slice) continue;
-                const int owner = static_cast<int>((v - c0) / a.slice);
-                const int64_t o0 = c0 + owner * a.slice;
-                const int olead = static_cast<int>((reinterpret_cast<uintptr_t>(x + o0) & 15u) / sizeof(T));
-                uint32_t addr;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;"
-                    : "=r"(addr)
-                    : "r"(base + static_cast<uint32_t>(v - o0 + olead) * 4), "r"(owner));
-                if (i < prompt) red_or_cluster(addr, 1u);
-                else red_add_cluster(addr, 2u);
-            }
-            __syncwarp();
-            cluster_sync();
-        }
-        for (int j0 = 0; j0 < nvec; j0 += kLogitBatch * kLogitThreads) {
-            if (j0 > 0) {
+        if (nb > 0) __syncthreads();  // an entry's number is settled before counts join it in the word
+        const int32_t* h = a.history + row * a.history_stride;
+        constexpr int kIds = 8;
+        for (int i0 = tid; i0 < hist; i0 += kIds * kLogitThreads) {
+            int id[kIds];
 #pragma unroll
-                for (int i = 0; i < kLogitBatch; ++i) {
-                    const int j = j0 + tid + i * kLogitThreads;
-                    if (j < nvec) batch[i] = load(j);
-                }
+            for (int k = 0; k < kIds; ++k) {
+                const int i = i0 + k * kLogitThreads;
+                id[k] = i < hist ? h[i] : -1;
             }
+#pragma unroll
+            for (int k = 0; k < kIds; ++k) {
+                if (id[k] < first || id[k] - first >= len) continue;
+                uint32_t* w = &words[id[k] - first + lead];
+                if (i0 + k * kLogitThreads < prompt) atomicOr(w, 1u);
+                else atomicAdd(w, 2u);
+            }
+        }
+        __syncthreads();
+    }
+    float best_v = 0.0f;  // the thread's best so far; its elements come in ascending order
+    int best_e = -1;
+    for (int j0 = 0; j0 < nvec; j0 += kLogitBatch * kLogitThreads) {
+        if (j0 > 0) {
 #pragma unroll
             for (int i = 0; i < kLogitBatch; ++i) {
                 const int j = j0 + tid + i * kLogitThreads;
-                if (j >= nvec) continue;
-                __align__(16) T v[kVec];
-                *reinterpret_cast<uint4*>(v) = batch[i];
-                const int64_t e = t0 - lead + static_cast<int64_t>(j) * kVec;
-                uint32_t w[kVec];
+                if (j < nvec) batch[i] = load(j);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kLogitBatch; ++i) {
+            const int j = j0 + tid + i * kLogitThreads;
+            if (j >= nvec) break;
+            __align__(16) T v[kVec];
+            *reinterpret_cast<uint4*>(v) = batch[i];
+            float f[kVec];
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) f[k] = LogitIo<T>::get(v[k]);
+            if (touched) {
+                uint32_t w[kVec], any = 0;
 #pragma unroll
                 for (int k = 0; k < kVec / 4; ++k)
-                    *reinterpret_cast<uint4*>(w + 4 * k) =
-                        touched ? reinterpret_cast<const uint4*>(words)[j * (kVec / 4) + k] : make_uint4(0, 0, 0, 0);
-                uint32_t allowed = 0xFFFFFFFFu;
-                if (mask) {  // bits e + begin .. + kVec (a first vector may begin before the slice)
-                    const int64_t g = e + a.begin < 0 ? 0 : e + a.begin;
-                    const uint32_t lo = mask[g >> 5];
-                    const int sh = static_cast<int>(g & 31);
-                    const uint32_t hi = sh + kVec > 32 && (g >> 5) + 1 < a.mask_words ? mask[(g >> 5) + 1] : 0u;
-                    allowed = __funnelshift_r(lo, hi, sh) << (g - (e + a.begin));
-                }
+                    *reinterpret_cast<uint4*>(w + 4 * k) = reinterpret_cast<const uint4*>(words)[j * (kVec / 4) + k];
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) {
-                    float f = LogitIo<T>::get(v[k]);
-                    if (w[k]) f = process_one(f, w[k], rep, pres, freq, a.bias_vals + b0);
-                    if (!((allowed >> k) & 1u)) f = -INFINITY;
-                    v[k] = LogitIo<T>::put(f);
-                    if (a.best || a.best_value) {
-                        if (e + k >= t0 && e + k < t1) {
-                            const uint64_t key = best_key(LogitIo<T>::get(v[k]), static_cast<uint32_t>(e + k));
-                            best = key > best ? key : best;
-                        }
-                    }
-                }
-                if (same && e >= t0 && e + kVec <= t1) {
-                    __stcs(reinterpret_cast<uint4*>(y + e), *reinterpret_cast<const uint4*>(v));
-                } else {
+                for (int k = 0; k < kVec; ++k) any |= w[k];
+                if (any) {
 #pragma unroll
                     for (int k = 0; k < kVec; ++k)
-                        if (e + k >= t0 && e + k < t1) y[e + k] = v[k];
+                        if (w[k]) f[k] = process_one(f[k], w[k], rep, pres, freq, a.bias_vals + b0);
+                }
+            }
+            if (mask) {
+                // (a first vector may begin before token 0, a last one end behind the last word: no tokens there)
+                const int at = first - lead + j * kVec, g = max(at, 0), sh = g & 31;
+                const uint32_t lo = mask[g >> 5];
+                const uint32_t hi = sh + kVec > 32 && (g >> 5) + 1 < a.mask_words ? mask[(g >> 5) + 1] : 0u;
+                const uint32_t allowed = __funnelshift_r(lo, hi, sh) << (g - at);
+#pragma unroll
+                for (int k = 0; k < kVec; ++k)
+                    if (!(allowed & (1u << k))) f[k] = -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) {
+                v[k] = LogitIo<T>::put(f[k]);
+                f[k] = LogitIo<T>::get(v[k]);
+            }
+            const bool inside = j >= full0 && j < full1;
+            if (inside && same) {
+                __stcs(reinterpret_cast<uint4*>(yb) + j, *reinterpret_cast<const uint4*>(v));
+            } else {
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) {
+                    const int e = j * kVec + k;
+                    if (e >= lead && e < lead + len) yb[e] = v[k];
+                }
+            }
+            // the first of the largest; once it is NaN it stays
+            float top = f[0];
+#pragma unroll
+            for (int k = 1; k < kVec; ++k) top = max_nan(top, f[k]);
+            if (best_e < 0 || !inside || (!(top <= best_v) && best_v == best_v)) {
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) {
+                    const int e = j * kVec + k;
+                    if (e >= lead && e < lead + len && (best_e < 0 || (!(f[k] <= best_v) && best_v == best_v))) {
+                        best_v = f[k];
+                        best_e = e;
+                    }
                 }
             }
         }
-        // the words are zeroed again for the next chunk, and no CTA counts into them before that: its
-        // cluster barrier after the zeroing
-        if (c + 1 < a.chunks && touched) __syncthreads();
     }
-    if (!a.best && !a.best_value) return;
+    if (!a.keys) return;
+    uint64_t best = best_e < 0 ? 0ull : best_key(best_v, static_cast<uint32_t>(t0 - lead) + static_cast<uint32_t>(best_e));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
@@ -278,63 +285,61 @@ __global__ void __launch_bounds__(kLogitThreads, 2) k_process_logits(const Logit
     __syncthreads();
     if (tid == 0) {
         for (int i = 1; i < kLogitThreads / 32; ++i) best = s_best[i] > best ? s_best[i] : best;
-        st_cluster_u64(dsmem_addr(&s_all[rank], 0), best);
+        a.keys[blockIdx.x] = best;
     }
-    __syncwarp();
-    cluster_sync();
-    if (rank == 0 && tid == 0) {
-        for (int i = 0; i < cn; ++i) best = s_all[i] > best ? s_all[i] : best;
-        const int64_t at = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
-        if (a.best) a.best[row] = at + a.begin;
-        if (a.best_value) {
-            const uint32_t ord = static_cast<uint32_t>(best >> 32);
+}
+
+// One warp per row: the best of its tiles.
+template <typename T>
+__global__ void __launch_bounds__(128) k_best_token(const uint64_t* __restrict__ keys, int64_t rows, int tiles,
+                                                    int64_t begin, int64_t* __restrict__ best, T* __restrict__ value) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t row = blockIdx.x * 4ll + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    uint64_t k = 0;
+    for (int i = threadIdx.x & 31; i < tiles; i += 32) {
+        const uint64_t other = keys[row * tiles + i];
+        k = other > k ? other : k;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t other = __shfl_xor_sync(0xffffffffu, k, o);
+        k = other > k ? other : k;
+    }
+    if ((threadIdx.x & 31) == 0) {
+        if (best) best[row] = begin + static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(k));
+        if (value) {
+            const uint32_t ord = static_cast<uint32_t>(k >> 32);
             const uint32_t bits = ord == 0xFFFFFFFFu ? 0x7FFFFFFFu : (ord & 0x80000000u) ? ord & 0x7FFFFFFFu : ~ord;
-            static_cast<T*>(a.best_value)[row] = LogitIo<T>::put(__uint_as_float(bits));
+            value[row] = LogitIo<T>::put(__uint_as_float(bits));
         }
     }
 }
 
-template <typename T>
-static cudaError_t launch_logits(LogitArgs a, int64_t rows, int sms, cudaStream_t s) {
-    // CTAs of a row: as many as its words need; more, down to slices of 2048 tokens, while the launch
-    // leaves SMs without their two CTAs
-    int cn = 1;
-    while (cn < kLogitMaxCluster && (a.vocab > static_cast<int64_t>(cn) * kLogitWords ||
-                                     (rows * cn < 2 * sms && a.vocab >= static_cast<int64_t>(cn) * 4096)))
-        cn *= 2;
-    constexpr int kVec = LogitIo<T>::kVec;
-    int64_t slice = ((a.vocab + cn - 1) / cn + kVec - 1) / kVec * kVec;
-    if (slice > kLogitWords) slice = kLogitWords;
-    a.slice = slice;
-    a.chunks = static_cast<int>((a.vocab + cn * slice - 1) / (cn * slice));
-    const size_t smem = static_cast<size_t>(slice + 2 * kVec) * 4;
-    static std::atomic<uint64_t> flags{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(flags.load() & bit)) {
-        e = cudaFuncSetAttribute(k_process_logits<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (kLogitWords + 2 * kVec) * 4);
-        if (e != cudaSuccess) return e;
-        flags.fetch_or(bit);
+// Tiles of a row: as many as fill the SMs (four CTAs each) a whole number of times with tiles that their words
+// allow, and none below kLogitMinTile tokens.
+static int logit_tiles(int64_t rows, int64_t vocab, int* tile) {
+    const int64_t slots = 4ll * sm_count();
+    int64_t tiles = 0;
+    for (int64_t k = 1; tiles * kLogitWords < vocab; ++k) {
+        tiles = k * slots / rows;
+        if (k > 64) tiles = (vocab + kLogitWords - 1) / kLogitWords;  // very many rows: nothing to balance
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows * cn));
-    cfg.blockDim = dim3(kLogitThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(cn);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return cudaLaunchKernelEx(&cfg, k_process_logits<T>, a);
+    const int64_t most = (vocab + kLogitMinTile - 1) / kLogitMinTile;
+    if (tiles > most) tiles = most;
+    *tile = static_cast<int>(((vocab + tiles - 1) / tiles + 7) / 8 * 8);
+    return static_cast<int>((vocab + *tile - 1) / *tile);
+}
+
+template <typename T>
+static cudaError_t launch_logits(const LogitArgs& a, int64_t rows, int64_t* best, void* value, cudaStream_t s) {
+    const size_t smem = static_cast<size_t>(a.tile + 2 * LogitIo<T>::kVec) * 4;
+    cudaError_t e = launch_pdl(k_process_logits<T>, dim3(static_cast<unsigned>(rows * a.tiles)), dim3(kLogitThreads), smem, s, a);
+    if (e == cudaSuccess && a.keys)
+        e = launch_pdl(k_best_token<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, s, a.keys, rows, a.tiles,
+                       a.begin, best, static_cast<T*>(value));
+    return e;
 }
 
 }  // namespace sc
@@ -343,21 +348,27 @@ using namespace sc;
 
 extern "C" {
 
+size_t sc_qwen2_process_logits_scratch(int64_t rows, int64_t vocab) {
+    if (rows <= 0 || rows > kLogitMaxRows || vocab <= 0 || vocab > (1ll << 30)) return 0;
+    int tile;
+    return static_cast<size_t>(rows) * logit_tiles(rows, vocab, &tile) * 8;
+}
+
 sc_status sc_qwen2_process_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
                                   int64_t vocab_begin, const int32_t* history, int64_t history_stride,
                                   const int32_t* prompt_len, const int32_t* hist_len, const float* repetition,
                                   const float* presence, const float* frequency, const int32_t* bias_ptr,
                                   const int32_t* bias_ids, const float* bias_vals, int64_t num_bias,
                                   const int32_t* mask, int64_t mask_words, int64_t mask_rows, const int32_t* mask_row,
-                                  void* out, int64_t out_stride, int64_t* best, void* best_value, uint32_t* status,
-                                  void* stream) {
+                                  void* out, int64_t out_stride, int64_t* best, void* best_value, void* scratch,
+                                  size_t scratch_bytes, uint32_t* status, void* stream) {
     auto bad = [](const char* what) {
         set_error(std::string("sc_qwen2_process_logits: ") + what);
         return SC_EINVAL;
     };
     if (dtype != SC_F32 && dtype != SC_F16 && dtype != SC_BF16) return bad("dtype is f32, f16 or bf16");
-    if (rows < 0 || vocab <= 0 || vocab > (1ll << 30) || rows > (1ll << 27)) return bad("rows or vocab out of range");
-    if (vocab_begin < 0 || vocab_begin > (1ll << 30)) return bad("vocab_begin out of range");
+    if (rows < 0 || vocab <= 0 || vocab > (1ll << 30) || rows > kLogitMaxRows) return bad("rows or vocab out of range");
+    if (vocab_begin < 0 || vocab_begin > (1ll << 30) - vocab) return bad("vocab_begin out of range");
     if (rows == 0) return SC_OK;
     if (!logits || !out) return bad("null logits or out");
     if (rows > 1 && (stride < vocab || out_stride < vocab)) return bad("rows overlap");
@@ -393,18 +404,21 @@ sc_status sc_qwen2_process_logits(const void* logits, int dtype, int64_t rows, i
     a.mask_row = mask_row;
     a.out = out;
     a.out_stride = out_stride;
-    a.best = best;
-    a.best_value = best_value;
     a.status = status;
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess) {
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
-        e = dtype == SC_F32 ? launch_logits<float>(a, rows, sms, s)
-            : dtype == SC_F16 ? launch_logits<__half>(a, rows, sms, s)
-                              : launch_logits<__nv_bfloat16>(a, rows, sms, s);
+    a.tiles = logit_tiles(rows, vocab, &a.tile);
+    if (rows * a.tiles > 0x7fffffff) return bad("rows or vocab out of range");
+    if (best || best_value) {
+        if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 8) return bad("scratch must be 8-byte aligned");
+        if (scratch_bytes < static_cast<size_t>(rows) * a.tiles * 8) {
+            set_error("sc_qwen2_process_logits: scratch too small");
+            return SC_ENOMEM;
+        }
+        a.keys = static_cast<uint64_t*>(scratch);
     }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = dtype == SC_F32   ? launch_logits<float>(a, rows, best, best_value, s)
+                          : dtype == SC_F16 ? launch_logits<__half>(a, rows, best, best_value, s)
+                                            : launch_logits<__nv_bfloat16>(a, rows, best, best_value, s);
     return e == cudaSuccess ? SC_OK : cuda_fail(e, "sc_qwen2_process_logits");
 }
 

@@ -200,7 +200,7 @@ cudaError_t paged_query_map(CUtensorMap* map, const PagedLaunch& a, int dtype, i
     return encode_map(map, a.q, dtype, dims, strides, box, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
-static int sm_count() {
+int sm_count() {
     static std::atomic<int> cache[64];
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;

@@ -9,7 +9,7 @@ import torch
 
 from ._lib import LIB
 from .op import _DT
-from .paged import _call, _status
+from .paged import _call, _size, _status
 
 
 def _vector(t: torch.Tensor, what: str, n: int, dtype: torch.dtype, dev: int) -> int:
@@ -94,13 +94,17 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
         p_mask = mask.data_ptr()
     elif mask_row is not None:
         raise ValueError("mask_row needs a mask")
-    best = value = None
+    best = value = scratch = None
+    nbytes = 0
     if return_best:
         best = logits.new_empty(rows, dtype=torch.int64)
         value = logits.new_empty(rows)
+        nbytes = _size(dev, "sc_qwen2_process_logits_scratch", rows, vocab)
+        scratch = best.new_empty(nbytes // 8)
     if rows > 0:
         _call(dev, LIB.sc_qwen2_process_logits, logits.data_ptr(), _DT[dtype], rows, vocab, stride, vocab_begin, p_hist,
               width, p_plen, p_hlen, p_rep, p_pres, p_freq, p_bptr, p_bids, p_bvals, nbias, p_mask, words, masks, p_mrow,
               out.data_ptr(), out_stride, None if best is None else best.data_ptr(),
-              None if value is None else value.data_ptr(), _status(status, dev))
+              None if value is None else value.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes,
+              _status(status, dev))
     return (out, best, value) if return_best else out

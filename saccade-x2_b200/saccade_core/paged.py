@@ -78,11 +78,10 @@ def _status(status: Optional[torch.Tensor], dev: int):
 
 
 @functools.lru_cache(maxsize=4096)
-def _scratch_bytes(dev: int, *sizes) -> int:
-    if dev == torch.cuda.current_device():
-        return int(LIB.sc_qwen2_paged_attention_scratch(*sizes))
+def _size(dev: int, name: str, *sizes) -> int:
+    """The answer of a scratch size function on device `dev`."""
     with torch.cuda.device(dev):
-        return int(LIB.sc_qwen2_paged_attention_scratch(*sizes))
+        return int(getattr(LIB, name)(*sizes))
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -153,7 +152,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lse = q.new_empty((tokens, nh), dtype=torch.float32) if return_lse else None
     if tokens > 0 and seqs > 0:
         max_q_len = min(int(max_q_len), tokens)
-        nbytes = _scratch_bytes(dev, tokens, seqs, nh, nkv, hd, max_q_len, _DT[dtype])
+        nbytes = _size(dev, "sc_qwen2_paged_attention_scratch", tokens, seqs, nh, nkv, hd, max_q_len, _DT[dtype])
         scratch = kv_len.new_empty((nbytes + 3) // 4)
         _call(dev, LIB.sc_qwen2_paged_attention, q.data_ptr(), qs, k_pages.data_ptr(), v_pages.data_ptr(), _DT[dtype], n,
               stride, page, block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(), kv_len.data_ptr(), seqs, tokens,
