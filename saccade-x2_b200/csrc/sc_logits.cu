@@ -14,6 +14,9 @@
 // other's shared memory measured slower: 39 us against 21 at 64 x 152064 f32 with 768 ids, two cluster barriers
 // and 31 clusters of 16 at a time.)
 //   word = (bias entry + 1) << 20 | n << 1 | in the prompt
+// Few tokens are touched, but nearly every warp of a streaming pass would meet one and take its division along, so
+// whoever counts a token first sets its bit in a map of the tile, the map's tokens are listed and processed by
+// themselves, their words replaced by the values, and the streaming pass looks at a vector's bits only.
 // Each CTA issues the loads of its first logits before it counts, so that they arrive meanwhile.  The best of
 // each tile goes to the scratch, and a second small kernel picks each row's.
 #include <atomic>
@@ -28,6 +31,9 @@ namespace sc {
 constexpr int kLogitThreads = 256;
 constexpr int kLogitWords = 10240;        // tokens of a tile at most (40 KB of words: four CTAs per SM)
 constexpr int kLogitMinTile = 2048;
+constexpr int kLogitMap = (kLogitWords + 16) / 32 + 1;
+constexpr int kLogitList = 1024;
+static_assert(kLogitMap <= 2 * kLogitThreads, "two words of the map per thread");
 constexpr int kLogitBatch = 6;            // 16-byte loads a thread has in flight
 constexpr int64_t kLogitMaxHistory = (1 << 19) - 1;  // 19 bits of a word count occurrences
 constexpr int64_t kLogitMaxRows = 1 << 20;
@@ -109,12 +115,16 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
     constexpr int kVec = LogitIo<T>::kVec;
     extern __shared__ __align__(16) uint32_t words[];  // one per token of the tile, from its first vector on
     __shared__ uint64_t s_best[kLogitThreads / 32];
+    __shared__ uint32_t s_map[kLogitMap];  // the tile's touched tokens
+    __shared__ uint16_t s_list[kLogitList];
+    __shared__ int s_sums[kLogitThreads / 32];
     pdl_launch_dependents();
-    const int64_t row = blockIdx.x / a.tiles;
+    const uint32_t row32 = blockIdx.x / static_cast<uint32_t>(a.tiles);
+    const int64_t row = row32;
     const int tid = threadIdx.x;
     // the tile's tokens [t0, t0 + len); vector j covers tokens t0 - lead + j * kVec .. + kVec, so that it starts on a
     // 16-byte boundary of the row; vectors [full0, full1) lie inside
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x - row * a.tiles) * a.tile;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x - row32 * a.tiles) * a.tile;
     const int len = static_cast<int>(imin64(a.vocab - t0, a.tile));
     const T* x = static_cast<const T*>(a.x) + row * a.stride + t0;
     const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
@@ -176,10 +186,15 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
     if (touched) {
         for (int i = tid; i < nvec * (kVec / 4); i += kLogitThreads)
             reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i <= nvec * kVec / 32; i += kLogitThreads) s_map[i] = 0;
         __syncthreads();
         for (int i = tid; i < nb; i += kLogitThreads) {
             const int v = a.bias_ids[b0 + i];
-            if (v >= first && v - first < len) atomicMax(&words[v - first + lead], static_cast<uint32_t>(i + 1) << 20);
+            if (v >= first && v - first < len) {
+                const int at = v - first + lead;
+                atomicMax(&words[at], static_cast<uint32_t>(i + 1) << 20);
+                atomicOr(&s_map[at >> 5], 1u << (at & 31));
+            }
         }
         if (nb > 0) __syncthreads();  // an entry's number is settled before counts join it in the word
         const int32_t* h = a.history + row * a.history_stride;
@@ -194,21 +209,68 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
 #pragma unroll
             for (int k = 0; k < kIds; ++k) {
                 if (id[k] < first || id[k] - first >= len) continue;
-                uint32_t* w = &words[id[k] - first + lead];
-                if (i0 + k * kLogitThreads < prompt) atomicOr(w, 1u);
-                else atomicAdd(w, 2u);
+                const int at = id[k] - first + lead;
+                if (i0 + k * kLogitThreads < prompt) atomicOr(&words[at], 1u);
+                else atomicAdd(&words[at], 2u);
+                atomicOr(&s_map[at >> 5], 1u << (at & 31));
             }
         }
         __syncthreads();
+        // the map's tokens as a list (thread t has words 2 t and 2 t + 1), kLogitList at a time, one thread each
+        const int lane = tid & 31, warp = tid >> 5, last = nvec * kVec / 32;
+        uint64_t mine = (2 * tid <= last ? s_map[2 * tid] : 0u) |
+                        static_cast<uint64_t>(2 * tid + 1 <= last ? s_map[2 * tid + 1] : 0u) << 32;
+        int upto = __popcll(mine);  // inclusive prefix sum over the block
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == 31) s_sums[warp] = upto;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int i = 0; i < kLogitThreads / 32; ++i) {
+            if (i < warp) upto += s_sums[i];
+            total += s_sums[i];
+        }
+        int place = upto - __popcll(mine);
+        for (int base = 0; base < total; base += kLogitList) {
+            for (; mine && place < base + kLogitList; mine &= mine - 1)
+                s_list[place++ - base] = static_cast<uint16_t>(64 * tid + __ffsll(static_cast<long long>(mine)) - 1);
+            __syncthreads();
+            for (int i = tid; i < min(total - base, kLogitList); i += kLogitThreads) {
+                const int at = s_list[i];
+                words[at] = __float_as_uint(process_one(LogitIo<T>::get(xb[at]), words[at], rep, pres, freq, a.bias_vals + b0));
+            }
+            __syncthreads();
+        }
     }
-    float best_v = 0.0f;  // the thread's best so far; its elements come in ascending order
-    int best_e = -1;
+    const bool even = first >= lead && ((first - lead) & (kVec - 1)) == 0;  // no vector's bits reach into the next word
+    auto mask_bits = [&](int j) {
+        // (a first vector may begin before token 0, a last one end behind the last word: no tokens there)
+        const int at = first - lead + j * kVec, g = max(at, 0), sh = g & 31;
+        const uint32_t lo = __ldg(mask + (g >> 5));
+        if (even) return lo >> sh;
+        const uint32_t hi = sh + kVec > 32 && (g >> 5) + 1 < a.mask_words ? __ldg(mask + (g >> 5) + 1) : 0u;
+        return __funnelshift_r(lo, hi, sh) << (g - at);
+    };
+    float best_v = 0.0f;  // the thread's best so far and the first vector it was in (they come in ascending order)
+    int best_j = -1;
     for (int j0 = 0; j0 < nvec; j0 += kLogitBatch * kLogitThreads) {
         if (j0 > 0) {
 #pragma unroll
             for (int i = 0; i < kLogitBatch; ++i) {
                 const int j = j0 + tid + i * kLogitThreads;
                 if (j < nvec) batch[i] = load(j);
+            }
+        }
+        uint32_t allow[kLogitBatch];  // each vector's mask bits
+        if (mask) {
+#pragma unroll
+            for (int i = 0; i < kLogitBatch; ++i) {
+                const int j = j0 + tid + i * kLogitThreads;
+                if (j < nvec) allow[i] = mask_bits(j);
             }
         }
 #pragma unroll
@@ -221,61 +283,46 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
 #pragma unroll
             for (int k = 0; k < kVec; ++k) f[k] = LogitIo<T>::get(v[k]);
             if (touched) {
-                uint32_t w[kVec], any = 0;
-#pragma unroll
-                for (int k = 0; k < kVec / 4; ++k)
-                    *reinterpret_cast<uint4*>(w + 4 * k) = reinterpret_cast<const uint4*>(words)[j * (kVec / 4) + k];
-#pragma unroll
-                for (int k = 0; k < kVec; ++k) any |= w[k];
-                if (any) {
+                const uint32_t bits = (s_map[j * kVec >> 5] >> (j * kVec & 31)) & ((1u << kVec) - 1u);
+                if (bits) {
 #pragma unroll
                     for (int k = 0; k < kVec; ++k)
-                        if (w[k]) f[k] = process_one(f[k], w[k], rep, pres, freq, a.bias_vals + b0);
+                        if (bits & (1u << k)) f[k] = __uint_as_float(words[j * kVec + k]);
                 }
             }
             if (mask) {
-                // (a first vector may begin before token 0, a last one end behind the last word: no tokens there)
-                const int at = first - lead + j * kVec, g = max(at, 0), sh = g & 31;
-                const uint32_t lo = mask[g >> 5];
-                const uint32_t hi = sh + kVec > 32 && (g >> 5) + 1 < a.mask_words ? mask[(g >> 5) + 1] : 0u;
-                const uint32_t allowed = __funnelshift_r(lo, hi, sh) << (g - at);
 #pragma unroll
                 for (int k = 0; k < kVec; ++k)
-                    if (!(allowed & (1u << k))) f[k] = -INFINITY;
+                    if (!(allow[i] & (1u << k))) f[k] = -INFINITY;
             }
 #pragma unroll
             for (int k = 0; k < kVec; ++k) {
                 v[k] = LogitIo<T>::put(f[k]);
                 f[k] = LogitIo<T>::get(v[k]);
             }
-            const bool inside = j >= full0 && j < full1;
-            if (inside && same) {
+            if (j >= full0 && j < full1 && same) {
                 __stcs(reinterpret_cast<uint4*>(yb) + j, *reinterpret_cast<const uint4*>(v));
             } else {
 #pragma unroll
                 for (int k = 0; k < kVec; ++k) {
                     const int e = j * kVec + k;
                     if (e >= lead && e < lead + len) yb[e] = v[k];
+                    else f[k] = -INFINITY;  // another tile's, or nobody's: no candidate
                 }
             }
-            // the first of the largest; once it is NaN it stays
             float top = f[0];
 #pragma unroll
             for (int k = 1; k < kVec; ++k) top = max_nan(top, f[k]);
-            if (best_e < 0 || !inside || (!(top <= best_v) && best_v == best_v)) {
-#pragma unroll
-                for (int k = 0; k < kVec; ++k) {
-                    const int e = j * kVec + k;
-                    if (e >= lead && e < lead + len && (best_e < 0 || (!(f[k] <= best_v) && best_v == best_v))) {
-                        best_v = f[k];
-                        best_e = e;
-                    }
-                }
+            // once it is NaN it stays
+            if (best_j < 0 || (!(top <= best_v) && best_v == best_v)) {
+                best_v = top;
+                best_j = j;
             }
         }
     }
     if (!a.keys) return;
-    uint64_t best = best_e < 0 ? 0ull : best_key(best_v, static_cast<uint32_t>(t0 - lead) + static_cast<uint32_t>(best_e));
+    const uint64_t mine = best_j < 0 ? 0ull : best_key(best_v, static_cast<uint32_t>(best_j));
+    uint64_t best = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
@@ -283,9 +330,17 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
     }
     if ((tid & 31) == 0) s_best[tid >> 5] = best;
     __syncthreads();
-    if (tid == 0) {
-        for (int i = 1; i < kLogitThreads / 32; ++i) best = s_best[i] > best ? s_best[i] : best;
-        a.keys[blockIdx.x] = best;
+    best = s_best[0];
+    for (int i = 1; i < kLogitThreads / 32; ++i) best = s_best[i] > best ? s_best[i] : best;
+    if (mine == best) {  // the one thread with that vector finds the token in what it has written
+        int at = -1;
+        for (int k = 0; k < kVec; ++k) {
+            const int e = best_j * kVec + k;
+            if (at >= 0 || e < lead || e >= lead + len) continue;
+            const float u = LogitIo<T>::get(yb[e]);
+            if (u == best_v || (u != u && best_v != best_v)) at = e;
+        }
+        a.keys[blockIdx.x] = best_key(best_v, static_cast<uint32_t>(t0 + at - lead));
     }
 }
 
