@@ -68,6 +68,7 @@ struct PagedCut {
     int64_t total, per;    // tiles in all, tiles per CTA
     int64_t first, left;   // this CTA's first tile and number of tiles
     int b, h, rt, tile;    // where the first one is
+    PagedSeq s;            // its sequence
 };
 
 __device__ __forceinline__ int paged_row_tiles(const PagedSeq& s, int tt) { return (s.q_len + tt - 1) / tt; }
@@ -120,7 +121,11 @@ __device__ __forceinline__ void paged_cut(const PagedKv& p, int64_t max_q, int t
         incl = scan(mine, &block);
         total += block;
     }
-    const int64_t per = total > 0 ? (total + gridDim.x - 1) / gridDim.x : 1;
+    // (32-bit divisions where they do: a 64-bit one costs a hundred instructions)
+    const bool small = total <= 0x7fffffff;
+    const int64_t per = total <= 0 ? 1
+                        : small    ? static_cast<int64_t>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x)
+                                   : (total + gridDim.x - 1) / gridDim.x;
     const int64_t first = per * blockIdx.x;
     if (tid == 0) {
         cut->total = total;
@@ -138,11 +143,13 @@ __device__ __forceinline__ void paged_cut(const PagedKv& p, int64_t max_q, int t
         if (rel >= incl - mine && rel < incl) {
             const int b = b0 + tid;
             const PagedSeq s = paged_seq(p, b, max_q);
-            const int64_t per_head = mine / p.nkv;
             int64_t at = rel - (incl - mine);
+            const int64_t per_head = small ? static_cast<uint32_t>(mine) / static_cast<uint32_t>(p.nkv) : mine / p.nkv;
+            const int h = static_cast<int>(small ? static_cast<uint32_t>(at) / static_cast<uint32_t>(per_head) : at / per_head);
+            at -= h * per_head;
+            cut->s = s;
             cut->b = b;
-            cut->h = static_cast<int>(at / per_head);
-            at %= per_head;
+            cut->h = h;
             int rt = 0;
             for (int n; at >= (n = paged_key_tiles(s, rt, tt, kt)); ++rt) at -= n;
             cut->rt = rt;
@@ -170,16 +177,11 @@ struct PagedWalk {
         at = c.first;
         left = c.left;
         t0 = t1 = tiles = 0;
-        s = PagedSeq{0, 0, 0};
-        fresh = true;
+        s = c.s;
     }
     // The next item, or false at the piece's end.
     __device__ __forceinline__ bool next(const PagedKv& p, int64_t max_q, int tt, int kt) {
         if (left <= 0) return false;
-        if (fresh) {
-            s = paged_seq(p, b, max_q);
-            fresh = false;
-        }
         if (++rt >= paged_row_tiles(s, tt)) {
             rt = 0;
             if (++h >= p.nkv) {
@@ -200,9 +202,6 @@ struct PagedWalk {
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
     __device__ __forceinline__ int slot() const { return t0 > 0 ? 0 : 1; }
-
-private:
-    bool fresh;
 };
 
 // What k_paged_combine joins: the item that CTA w begins and does not finish (pieces 0: none).
@@ -277,6 +276,10 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 __device__ __forceinline__ void tma_page(void* smem_dst, const CUtensorMap* map, int col, int row, int head, int page,

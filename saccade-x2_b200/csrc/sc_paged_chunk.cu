@@ -45,6 +45,50 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* r) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// Waits for the loads of `r`, which no use of it may pass.
+__device__ __forceinline__ void tc_wait_ld32(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 16 lanes x 32 columns: lane (g, c) = (lane / 4, lane % 4) gets, per 8 columns k, columns 8 k + 2 c and + 1 of TMEM lanes
+// g (r[4 k], r[4 k + 1]) and g + 8 (r[4 k + 2], r[4 k + 3]); waits for them.
+__device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Lane c of each four gives p[k] to lane k and gets p[c] of lane k as p[k].
+__device__ __forceinline__ void quad_transpose(uint32_t (&p)[4], int c) {
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k & d) continue;
+            const bool up = c & d;  // keeps p[k + d], gives p[k]
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? p[k] : p[k + d], d);
+            if (up) p[k] = got;
+            else p[k + d] = got;
+        }
+}
 // D[128 x N] (+)= A[128 x 16] * B[16 x N], both operands in shared memory.
 __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                           uint32_t accumulate) {
@@ -117,6 +161,11 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
         mbar_init(&done, 1);
         fence_mbar_init();
     }
+    if (tid == 32 * 8) {
+        prefetch_map(&P.qmap);
+        prefetch_map(&P.kmap);
+        prefetch_map(&P.vmap);
+    }
     if (warp == 9) {
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
@@ -167,55 +216,80 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_full[half], count & 1, kv.status));
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t sr[128];
+                const bool edge = k0 + C::kKeys > first_pos + 1;
+                const int lim = pos - k0;  // columns up to it are attended
+                auto mask = [&](uint32_t* v, int c) {
+                    if (edge) {
+                        const int x = lim - 32 * c;
+                        const uint32_t live = x >= 31 ? 0xFFFFFFFFu : x < 0 ? 0u : (2u << x) - 1u;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, sr + 32 * i);
-                tc_wait_ld();
-                if (k0 + C::kKeys > first_pos + 1) {
-                    const int lim = pos - k0;  // columns up to it are attended
+                        for (int i = 0; i < 32; ++i)
+                            if (!(live & (1u << i))) v[i] = 0xFF800000u;  // -inf
+                    }
+                };
+                // P against the reference as it is, and the row's maximum beside it, 32 columns at a time while the
+                // next 32 are loaded.  A row without a reference takes the first columns' maximum for one; a row that
+                // has left its reference too far takes its own maximum, and P is computed once more.
+                uint32_t pk[64];
+                float part[2];
+                for (;;) {
+                    const uint64_t sl = pair(sl2, sl2);
+                    uint64_t mm = 0, sum[2] = {0, 0};
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    uint32_t v[2][32];
+                    tc_ld32(ts, v[0]);
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i > lim) sr[i] = 0xFF800000u;  // -inf
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t* x = v[c & 1];
+                        tc_wait_ld32(x);
+                        if (c < 3) tc_ld32(ts + 32 * (c + 1), v[(c + 1) & 1]);
+                        mask(x, c);
 #pragma unroll
-                for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(sr[i]));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-                if (__any_sync(0xffffffffu, top > m + kMove)) {
-                    const float mn = top > m + kMove ? top - kShift : m;  // each row by itself
-                    if (j > 0) {
-                        const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
-                        l *= f;
-                        if (__any_sync(0xffffffffu, f != 1.0f)) {
+                        for (int i = 0; i < 16; ++i)
+                            mx[i & 1] = max3(mx[i & 1], __uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+                        if (c == 0) {
+                            if (m == -INFINITY) m = fmaxf(mx[0], mx[1]) * sl2 - kShift;
+                            const float ms = m == -INFINITY ? 0.0f : m;
+                            mm = pair(-ms, -ms);
+                        }
 #pragma unroll
-                            for (int c = 0; c < kHd; c += 32) {
-                                uint32_t o[32];
-                                tc_ld32(to + c, o);
-                                tc_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                tc_st32(to + c, o);
-                            }
+                        for (int i = 0; i < 16; ++i) {
+                            uint64_t t;
+                            asm("fma.rn.f32x2 %0, %1, %2, %3;"
+                                : "=l"(t)
+                                : "l"(pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]))), "l"(sl), "l"(mm));
+                            float e0, e1;
+                            asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(t));
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum[i & 1]) : "l"(pair(e0, e1)));
+                            pk[16 * c + i] = M::pack(e0, e1);
                         }
                     }
+                    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum[0]) : "l"(sum[1]));
+                    asm("mov.b64 {%0, %1}, %2;" : "=f"(part[0]), "=f"(part[1]) : "l"(sum[0]));
+                    const float top = fmaxf(mx[0], mx[1]) * sl2;
+                    const bool move = top > m + kMove;
+                    if (!__any_sync(0xffffffffu, move)) break;
+                    const float mn = move ? top - kShift : m;  // each row by itself
+                    const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
+                    l *= f;
                     m = mn;
-                }
-                const float ms = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < kHd; c += 32) {
+                            uint32_t o[32];
+                            tc_ld32(to + c, o);
+                            tc_wait_ld32(o);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float a = ex2(fmaf(__uint_as_float(sr[64 * c + 2 * i]), sl2, -ms));
-                        const float b = ex2(fmaf(__uint_as_float(sr[64 * c + 2 * i + 1]), sl2, -ms));
-                        sum[i & 1] += a;
-                        sum[2 + (i & 1)] += b;
-                        pk[i] = M::pack(a, b);
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tc_st32(to + c, o);
+                        }
                     }
-                    tc_st32(ts + 32 * c, pk);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l += part[0] + part[1];
+                tc_st32(ts, pk);
+                tc_st32(ts + 32, pk + 32);
                 if (half == 0 && k0 + C::kKeys > keys) {
                     // V rows behind the item's last position hold whatever was there: 0 * NaN must not be
                     const int vt = it + 2 * j + 1, from = max(0, keys - k0);
@@ -238,34 +312,48 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
             if (!ok) break;
             tc_fence_after();
             const bool whole = w.whole();
-            const int64_t orow = (w.s.row0 + (tok < 0 ? 0 : tok)) * kv.nh + w.h * G + g;
-            const int64_t srow = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * 256 + half * 128 + row;
+            const int orow = tok < 0 ? -1 : static_cast<int>((w.s.row0 + tok) * kv.nh) + w.h * G + g;
+            const int64_t slot_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * 256 + half * 128 + 32 * (warp & 3);
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            // 16 rows x 32 columns at a time, four lanes to a row (a lane per row would touch 32 lines with
+            // every store): lane (g4, c4) has columns 8 k + 2 c4 .. + 1 of rows g4 and g4 + 8
+            const int g4 = lane >> 2, c4 = lane & 3;
 #pragma unroll
-            for (int c = 0; c < kHd; c += 32) {
-                uint32_t o[32];
-                tc_ld32(to + c, o);
-                tc_wait_ld();
-                if (tok < 0) continue;
-                if (whole) {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(A.o.out) + orow * kHd + c);
+            for (int r0 = 0; r0 < 32; r0 += 16) {
+                const int or0 = __shfl_sync(0xffffffffu, orow, r0 + g4), or1 = __shfl_sync(0xffffffffu, orow, r0 + g4 + 8);
+                const float in0 = __shfl_sync(0xffffffffu, inv, r0 + g4), in1 = __shfl_sync(0xffffffffu, inv, r0 + g4 + 8);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t p[4];
+                for (int c = 0; c < kHd; c += 32) {
+                    uint32_t o[16];
+                    tc_ld_16x32(to + (static_cast<uint32_t>(r0) << 16) + c, o);
+                    if (whole) {
+                        uint32_t p0[4], p1[4];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            p[x] = M::pack(__uint_as_float(o[8 * i + 2 * x]) * inv, __uint_as_float(o[8 * i + 2 * x + 1]) * inv);
-                        dst[i] = make_uint4(p[0], p[1], p[2], p[3]);
+                        for (int k = 0; k < 4; ++k) {
+                            p0[k] = M::pack(__uint_as_float(o[4 * k]) * in0, __uint_as_float(o[4 * k + 1]) * in0);
+                            p1[k] = M::pack(__uint_as_float(o[4 * k + 2]) * in1, __uint_as_float(o[4 * k + 3]) * in1);
+                        }
+                        quad_transpose(p0, c4);  // lane c4 now has columns 8 c4 .. + 7
+                        quad_transpose(p1, c4);
+                        if (or0 >= 0)
+                            *reinterpret_cast<uint4*>(static_cast<T*>(A.o.out) + static_cast<int64_t>(or0) * kHd + c + 8 * c4) =
+                                make_uint4(p0[0], p0[1], p0[2], p0[3]);
+                        if (or1 >= 0)
+                            *reinterpret_cast<uint4*>(static_cast<T*>(A.o.out) + static_cast<int64_t>(or1) * kHd + c + 8 * c4) =
+                                make_uint4(p1[0], p1[1], p1[2], p1[3]);
+                    } else {
+                        float* dst = A.sc.o + (slot_row + r0 + g4) * kHd + c + 2 * c4;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if (or0 >= 0) *reinterpret_cast<uint2*>(dst + 8 * k) = make_uint2(o[4 * k], o[4 * k + 1]);
+                            if (or1 >= 0) *reinterpret_cast<uint2*>(dst + 8 * kHd + 8 * k) = make_uint2(o[4 * k + 2], o[4 * k + 3]);
+                        }
                     }
-                } else {
-                    uint4* dst = reinterpret_cast<uint4*>(A.sc.o + srow * kHd + c);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
             }
             tc_fence_before();
             if (tok >= 0) {
-                if (!whole) *reinterpret_cast<float2*>(A.sc.ml + srow * 2) = make_float2(m, l);
+                if (!whole) *reinterpret_cast<float2*>(A.sc.ml + (slot_row + lane) * 2) = make_float2(m, l);
                 else if (A.o.lse) A.o.lse[orow] = l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
             }
         }
@@ -275,13 +363,26 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) {
             // ---------------- loads: the whole warp, a box per lane
-            int it = 0, item = 0, issued = 0;  // ring tiles (K and V count), items
+            int it = 0, item = 0, issued = 0, queries = 0;  // ring tiles (K and V count), items, loads of each
             bool stop = false;
             while (!stop && w.next(kv, A.max_q, tt, C::kKeys)) {
                 const int shift = kv.page_shift, bs = P.box_shift;
                 const int keys = w.s.kv_len - w.s.q_len + min((w.rt + 1) * tt, w.s.q_len);
                 const int32_t* table = kv.table + w.b * kv.max_pages;
                 int have = -1, id = 0;  // pages have .. have + 31 of the sequence, one per lane
+                auto load_q = [&]() {
+                    const bool two = w.rt * tt + per < w.s.q_len;
+                    const int parts = (two ? 2 : 1) * C::kBlocks;
+                    if (lane == 0) mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(parts) * G * per * 128u);
+                    __syncwarp();
+                    if (lane < parts) {
+                        const int half = lane / C::kBlocks, blk = lane % C::kBlocks;
+                        tma_page(smem + half * C::kTile + blk * C::kBlock, &P.qmap, blk * 64, 0, w.h,
+                                 static_cast<int>(w.s.row0) + w.rt * tt + half * per, &q_full);
+                    }
+                    ++queries;
+                };
+                if (item == 0) load_q();
                 for (int t = w.t0; t < w.t1 && !stop; ++t) {
                     const int k0 = t * C::kKeys, n = max(0, min(C::kKeys, keys - k0));
                     const int boxes = (n + (1 << bs) - 1) >> bs;
@@ -318,31 +419,21 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                                          key & ((1 << shift) - 1), w.h, page, &kv_full[sl]);
                         }
                     }
-                    if (t == w.t0 && !stop) {
+                    if (t == w.t0 && item > 0 && !stop) {
                         // the item's queries, after its first keys: the item before may still be read
-                        if (item > 0 && !mbar_wait(&q_empty, (item - 1) & 1, kv.status)) stop = true;
+                        if (!mbar_wait(&q_empty, (item - 1) & 1, kv.status)) stop = true;
                         stop = __any_sync(0xffffffffu, stop);
-                        if (!stop) {
-                            const bool two = w.rt * tt + per < w.s.q_len;
-                            const int parts = (two ? 2 : 1) * C::kBlocks;
-                            if (lane == 0)
-                                mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(parts) * G * per * 128u);
-                            __syncwarp();
-                            if (lane < parts) {
-                                const int half = lane / C::kBlocks, blk = lane % C::kBlocks;
-                                tma_page(smem + half * C::kTile + blk * C::kBlock, &P.qmap, blk * 64, 0, w.h,
-                                         static_cast<int>(w.s.row0) + w.rt * tt + half * per, &q_full);
-                            }
-                            ++item;
-                        }
+                        if (!stop) load_q();
                     }
                 }
+                ++item;
             }
+
             // copies in flight end before the block does
             if (lane == 0) {
                 for (int i = issued > C::kSlots ? issued - C::kSlots : 0; i < issued; ++i)
                     mbar_wait(&kv_full[i % C::kSlots], (i / C::kSlots) & 1, nullptr, kDrainNs);
-                if (item > 0) mbar_wait(&q_full, (item - 1) & 1, nullptr, kDrainNs);
+                if (queries > 0) mbar_wait(&q_full, (queries - 1) & 1, nullptr, kDrainNs);
             }
             __syncwarp();
         } else if (warp == 9) {
@@ -382,11 +473,11 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                 for (int j = 0; j < n && ok; ++j) {
                     const int vt = it + 2 * j + 1, kt = vt + 1;  // ring tiles of V(j) and K(j + 1)
                     if (!wait(&kv_full[vt % C::kSlots], (vt / C::kSlots) & 1)) break;
+                    if (j + 1 < n && !wait(&kv_full[kt % C::kSlots], (kt / C::kSlots) & 1)) break;
                     for (int half = 0; half < (two ? 2 : 1); ++half) {
                         if (!wait(&p_full[half], pcount[half] & 1)) break;
                         ++pcount[half];
-                        if (half == 0 && j + 1 < n && !wait(&kv_full[kt % C::kSlots], (kt / C::kSlots) & 1)) break;
-                        tc_fence_after();
+                            tc_fence_after();
                         const bool end = half == (two ? 1 : 0);
                         if (elect_one()) {
                             const uint32_t b = chunk_low(ra + (vt % C::kSlots) * C::kTile, C::kBlock);

@@ -78,6 +78,10 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
     const PagedKv& kv = A.c;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = kv.nh / kv.nkv, tt = A.tl.tt;
+    if (tid == 32 * C::kWarps) {
+        prefetch_map(&P.kmap);
+        prefetch_map(&P.vmap);
+    }
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&full[i], 1);
