@@ -164,12 +164,15 @@ __device__ __forceinline__ void paged_cut(const PagedKv& p, int64_t max_q, int t
 struct PagedWalk {
     PagedSeq s;
     int b, h, rt;
+    int rts;        // row tiles of the sequence
     int tiles;      // key tiles of the item
     int t0, t1;     // the piece's share of them
     int64_t at, left;
     int next_tile;
 
-    __device__ __forceinline__ void begin(const PagedCut& c) {
+    __device__ __forceinline__ void begin(const PagedCut& c, int tt) {
+        s = c.s;
+        rts = c.left > 0 ? paged_row_tiles(s, tt) : 0;
         b = c.b;
         h = c.h;
         rt = c.rt - 1;
@@ -177,12 +180,11 @@ struct PagedWalk {
         at = c.first;
         left = c.left;
         t0 = t1 = tiles = 0;
-        s = c.s;
     }
     // The next item, or false at the piece's end.
     __device__ __forceinline__ bool next(const PagedKv& p, int64_t max_q, int tt, int kt) {
         if (left <= 0) return false;
-        if (++rt >= paged_row_tiles(s, tt)) {
+        if (++rt >= rts) {
             rt = 0;
             if (++h >= p.nkv) {
                 h = 0;
@@ -190,6 +192,7 @@ struct PagedWalk {
                     if (++b >= p.num_seqs) return false;
                     s = paged_seq(p, b, max_q);
                 } while (s.q_len == 0);
+                rts = paged_row_tiles(s, tt);
             }
         }
         tiles = paged_key_tiles(s, rt, tt, kt);
@@ -241,14 +244,21 @@ struct PagedOut {
     float sl2;             // scale * log2(e)
 };
 
-// Row r of a row tile: its token in the sequence and its query head of the group, or token -1.
-__device__ __forceinline__ int paged_row_token(int r, int sub, int group, int rt, int tt, int q_len, int* g) {
-    const int per = sub / group, half = r / sub, x = r - half * sub;
-    const int tok = x / group;
-    *g = x - tok * group;
-    const int t = rt * tt + half * per + tok;
-    return tok < per && t < q_len ? t : -1;
-}
+// Row r of a row tile is token `tok` of the tile (beyond every sequence: none) and query head `g` of the group,
+// whatever the item: the divisions are done once.
+struct PagedRow {
+    int tok, g;
+    __device__ __forceinline__ PagedRow(int r, int sub, int group) {
+        const int per = sub / group, half = r / sub, x = r - half * sub;
+        const int t = x / group;
+        g = x - t * group;
+        tok = t < per ? half * per + t : 1 << 30;
+    }
+    // The row's token in the sequence, or -1.
+    __device__ __forceinline__ int token(int rt, int tt, int q_len) const {
+        return tok < q_len - rt * tt ? rt * tt + tok : -1;
+    }
+};
 
 // Two f32 as two 16-bit values of the cache's type, and back.
 template <typename T>

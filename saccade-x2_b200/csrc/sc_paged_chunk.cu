@@ -66,15 +66,23 @@ __device__ __forceinline__ uint64_t pair(float a, float b) {
     return r;
 }
 // 16 lanes x 32 columns: lane (g, c) = (lane / 4, lane % 4) gets, per 8 columns k, columns 8 k + 2 c and + 1 of TMEM lanes
-// g (r[4 k], r[4 k + 1]) and g + 8 (r[4 k + 2], r[4 k + 3]); waits for them.
+// g (r[4 k], r[4 k + 1]) and g + 8 (r[4 k + 2], r[4 k + 3]).
 __device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld16x2(uint32_t (&a)[16], uint32_t (&b)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]), "+r"(a[8]),
+                   "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]), "+r"(b[0]),
+                   "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]), "+r"(b[6]), "+r"(b[7]), "+r"(b[8]),
+                   "+r"(b[9]), "+r"(b[10]), "+r"(b[11]), "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15])
+                 :
+                 : "memory");
 }
 // Lane c of each four gives p[k] to lane k and gets p[c] of lane k as p[k].
 __device__ __forceinline__ void quad_transpose(uint32_t (&p)[4], int c) {
@@ -178,7 +186,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
     pdl_wait();
     paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);  // synchronises the block
     PagedWalk w;
-    w.begin(cut);
+    w.begin(cut, tt);
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -192,6 +200,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
         int it = 0;              // ring tiles, as the loads count them
         uint32_t count = 0, items = 0;
         bool ok = true;
+        const PagedRow mine(half * 128 + row, 128, G);
         PagedJoin join{0, 0, 0, 0, 0};
         while (ok && w.next(kv, A.max_q, tt, C::kKeys)) {
             const int n = w.t1 - w.t0;
@@ -204,8 +213,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                 // a cut item's second half is empty: its rows are never joined
                 continue;
             }
-            int g;
-            const int tok = paged_row_token(half * 128 + row, 128, G, w.rt, tt, w.s.q_len, &g);
+            const int tok = mine.token(w.rt, tt, w.s.q_len);
             const int start = w.s.kv_len - w.s.q_len;
             const int pos = tok >= 0 ? start + tok : -1;
             const int first_pos = start + w.rt * tt + half * per;  // the least position of the half's rows
@@ -312,43 +320,48 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
             if (!ok) break;
             tc_fence_after();
             const bool whole = w.whole();
-            const int orow = tok < 0 ? -1 : static_cast<int>((w.s.row0 + tok) * kv.nh) + w.h * G + g;
+            const int orow = tok < 0 ? -1 : static_cast<int>((w.s.row0 + tok) * kv.nh) + w.h * G + mine.g;
             const int64_t slot_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * 256 + half * 128 + 32 * (warp & 3);
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             // 16 rows x 32 columns at a time, four lanes to a row (a lane per row would touch 32 lines with
             // every store): lane (g4, c4) has columns 8 k + 2 c4 .. + 1 of rows g4 and g4 + 8
             const int g4 = lane >> 2, c4 = lane & 3;
+            int orows[4];
+            float invs[4];
 #pragma unroll
-            for (int r0 = 0; r0 < 32; r0 += 16) {
-                const int or0 = __shfl_sync(0xffffffffu, orow, r0 + g4), or1 = __shfl_sync(0xffffffffu, orow, r0 + g4 + 8);
-                const float in0 = __shfl_sync(0xffffffffu, inv, r0 + g4), in1 = __shfl_sync(0xffffffffu, inv, r0 + g4 + 8);
+            for (int i = 0; i < 4; ++i) {
+                orows[i] = __shfl_sync(0xffffffffu, orow, 8 * i + g4);
+                invs[i] = __shfl_sync(0xffffffffu, inv, 8 * i + g4);
+            }
+            // (rolled: what runs once per item should not push the softmax out of the instruction cache)
+#pragma unroll 1
+            for (int c = 0; c < kHd; c += 32) {
+                uint32_t o[2][16];
+                tc_ld_16x32(to + c, o[0]);
+                tc_ld_16x32(to + (16u << 16) + c, o[1]);
+                tc_wait_ld16x2(o[0], o[1]);
+                if (whole) {
 #pragma unroll
-                for (int c = 0; c < kHd; c += 32) {
-                    uint32_t o[16];
-                    tc_ld_16x32(to + (static_cast<uint32_t>(r0) << 16) + c, o);
-                    if (whole) {
-                        uint32_t p0[4], p1[4];
+                    for (int i = 0; i < 4; ++i) {  // rows g4 + 8 i
+                        const uint32_t* x = o[i >> 1] + 2 * (i & 1);
+                        uint32_t p[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            p0[k] = M::pack(__uint_as_float(o[4 * k]) * in0, __uint_as_float(o[4 * k + 1]) * in0);
-                            p1[k] = M::pack(__uint_as_float(o[4 * k + 2]) * in1, __uint_as_float(o[4 * k + 3]) * in1);
-                        }
-                        quad_transpose(p0, c4);  // lane c4 now has columns 8 c4 .. + 7
-                        quad_transpose(p1, c4);
-                        if (or0 >= 0)
-                            *reinterpret_cast<uint4*>(static_cast<T*>(A.o.out) + static_cast<int64_t>(or0) * kHd + c + 8 * c4) =
-                                make_uint4(p0[0], p0[1], p0[2], p0[3]);
-                        if (or1 >= 0)
-                            *reinterpret_cast<uint4*>(static_cast<T*>(A.o.out) + static_cast<int64_t>(or1) * kHd + c + 8 * c4) =
-                                make_uint4(p1[0], p1[1], p1[2], p1[3]);
-                    } else {
-                        float* dst = A.sc.o + (slot_row + r0 + g4) * kHd + c + 2 * c4;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if (or0 >= 0) *reinterpret_cast<uint2*>(dst + 8 * k) = make_uint2(o[4 * k], o[4 * k + 1]);
-                            if (or1 >= 0) *reinterpret_cast<uint2*>(dst + 8 * kHd + 8 * k) = make_uint2(o[4 * k + 2], o[4 * k + 3]);
-                        }
+                        for (int k = 0; k < 4; ++k)
+                            p[k] = M::pack(__uint_as_float(x[4 * k]) * invs[i], __uint_as_float(x[4 * k + 1]) * invs[i]);
+                        quad_transpose(p, c4);  // lane c4 now has columns 8 c4 .. + 7
+                        if (orows[i] >= 0)
+                            *reinterpret_cast<uint4*>(static_cast<T*>(A.o.out) + static_cast<int64_t>(orows[i]) * kHd + c +
+                                                      8 * c4) = make_uint4(p[0], p[1], p[2], p[3]);
                     }
+                } else {
+                    float* dst = A.sc.o + (slot_row + g4) * kHd + c + 2 * c4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (orows[i] >= 0)
+                                *reinterpret_cast<uint2*>(dst + 8 * i * kHd + 8 * k) =
+                                    make_uint2(o[i >> 1][4 * k + 2 * (i & 1)], o[i >> 1][4 * k + 2 * (i & 1) + 1]);
                 }
             }
             tc_fence_before();

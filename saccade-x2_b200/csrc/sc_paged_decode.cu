@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
     pdl_wait();
     paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);  // synchronises the block
     PagedWalk w;
-    w.begin(cut);
+    w.begin(cut, tt);
 
     if (warp == C::kWarps) {
         // ---- producer: the whole warp, a box per lane
@@ -161,20 +161,21 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
     // V matrices (keys 0-7, dims 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
     const int kkey = 16 * warp + (lane >> 4) * 8 + (lane & 7), kchunk = (lane >> 3) & 1;
     const int vkey = 16 * warp + ((lane >> 3) & 1) * 8 + (lane & 7), vchunk = lane >> 4;
+    const PagedRow rows[2] = {PagedRow(g4, 16, G), PagedRow(g4 + 8, 16, G)}, written(tid >> 3, 16, G);
     PagedJoin join{0, 0, 0, 0, 0};
     int it = 0;
     bool late = false;
     while (w.next(kv, A.max_q, tt, C::kKeys)) {
         // this thread's two rows
-        int gr[2], tok[2];
+        int tok[2];
         uint32_t qa[kSteps][4];
         int pos[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            tok[r] = paged_row_token(g4 + 8 * r, 16, G, w.rt, tt, w.s.q_len, &gr[r]);
+            tok[r] = rows[r].token(w.rt, tt, w.s.q_len);
             pos[r] = tok[r] >= 0 ? w.s.kv_len - w.s.q_len + tok[r] : -1;
             const T* src = static_cast<const T*>(A.q) + (w.s.row0 + (tok[r] < 0 ? 0 : tok[r])) * A.q_stride +
-                           (w.h * G + gr[r]) * kHd + 2 * c4;
+                           (w.h * G + rows[r].g) * kHd + 2 * c4;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
@@ -301,9 +302,8 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
         for (int i = 0; i < C::kWarps; ++i) mm = fmaxf(mm, s_m[i][row]);
 #pragma unroll
         for (int i = 0; i < C::kWarps; ++i) ll += s_m[i][row] == -INFINITY ? 0.0f : s_l[i][row] * ex2(s_m[i][row] - mm);
-        int og;
-        const int ot = paged_row_token(row, 16, G, w.rt, tt, w.s.q_len, &og);
-        const int64_t orow = (w.s.row0 + (ot < 0 ? 0 : ot)) * kv.nh + w.h * G + og;
+        const int ot = written.token(w.rt, tt, w.s.q_len);
+        const int64_t orow = (w.s.row0 + (ot < 0 ? 0 : ot)) * kv.nh + w.h * G + written.g;
         const bool whole = w.whole();
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + w.slot();
         const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(256) k_paged_combine(const PagedLaunch A) {
     const int G = A.c.nh / A.c.nkv, rows = A.tl.rows;
     constexpr int kCols = kHd / 16;  // columns of a thread
     const int row = blockIdx.y * kCombineRows + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * kCols;
-    int g;
-    const int tok = paged_row_token(row, A.tl.sub, G, j.rt, A.tl.tt, j.q_len, &g);
+    const PagedRow mine(row, A.tl.sub, G);
+    const int tok = mine.token(j.rt, A.tl.tt, j.q_len);
     if (tok < 0) return;
     // piece i: slot 1 of CTA w for the first, slot 0 of CTA w + i for the others
     auto slot = [&](int i) { return static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(256) k_paged_combine(const PagedLaunch A) {
             }
         }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int64_t orow = (j.row0 + tok) * A.c.nh + j.h * G + g;
+    const int64_t orow = (j.row0 + tok) * A.c.nh + j.h * G + mine.g;
     Out* dst = static_cast<Out*>(A.o.out) + orow * kHd + c0;
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {

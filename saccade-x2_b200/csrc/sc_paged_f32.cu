@@ -65,7 +65,9 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
     pdl_wait();
     paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);
     PagedWalk w;
-    w.begin(cut);
+    w.begin(cut, tt);
+    const PagedRow mine[4] = {PagedRow(ty * 4, kRows, G), PagedRow(ty * 4 + 1, kRows, G), PagedRow(ty * 4 + 2, kRows, G),
+                              PagedRow(ty * 4 + 3, kRows, G)};
     PagedJoin join{0, 0, 0, 0, 0};
     const float sl2 = A.o.sl2;
     while (w.next(kv, A.max_q, tt, C::kKeys)) {
@@ -96,19 +98,18 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
         load(kv.v, sv, w.t0);
         for (int i = tid; i < kRows * (kHd / 4); i += C::kThreads) {
             const int r = i / (kHd / 4), c = i % (kHd / 4);
-            int g;
-            const int tok = paged_row_token(r, kRows, G, w.rt, tt, w.s.q_len, &g);
+            const PagedRow row(r, kRows, G);
+            const int tok = row.token(w.rt, tt, w.s.q_len);
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (tok >= 0)
                 v = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + (w.s.row0 + tok) * A.q_stride +
-                                                     (w.h * G + g) * kHd + c * 4);
+                                                     (w.h * G + row.g) * kHd + c * 4);
             *reinterpret_cast<float4*>(sq + r * C::kLd + c * 4) = v;
         }
         int pos[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            int g;
-            const int tok = paged_row_token(ty * 4 + i, kRows, G, w.rt, tt, w.s.q_len, &g);
+            const int tok = mine[i].token(w.rt, tt, w.s.q_len);
             pos[i] = tok >= 0 ? start + tok : -1;
         }
         float m[4], l[4];
@@ -216,10 +217,10 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
         const bool whole = w.whole();
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + w.slot();
         auto write = [&](int row, int col, float4 v, float mm, float ll) {  // 4 columns of a row, and its sums once
-            int g;
-            const int tok = paged_row_token(row, kRows, G, w.rt, tt, w.s.q_len, &g);
+            const PagedRow r(row, kRows, G);
+            const int tok = r.token(w.rt, tt, w.s.q_len);
             if (tok < 0) return;
-            const int64_t orow = (w.s.row0 + tok) * kv.nh + w.h * G + g;
+            const int64_t orow = (w.s.row0 + tok) * kv.nh + w.h * G + r.g;
             if (whole) {
                 const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
                 v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
