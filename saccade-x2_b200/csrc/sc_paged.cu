@@ -34,7 +34,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 // A thread has 8 rotated pairs (elements d..d+7 and d+hd/2..d+hd/2+7) of one token and takes the
 // heads in turn, so that the token's angles are loaded once for all of its heads; q, k and v heads
 // follow one another in the loop.  Bytes bound: q, k, v read, q' and the cache rows written, two
-// table rows per token.
+// table rows per token.  The loads of the first heads do not depend on the token's place: they are issued before
+// it is looked up, and kBatch heads' loads are on their way at a time.
 constexpr int kAppendThreads = 256;
 
 struct AppendArgs {
@@ -51,19 +52,19 @@ struct AppendArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&f)[8]) {
-    if (vec) {
-        __align__(16) T t[8];
+struct Eight {  // 8 consecutive values as they are in memory
+    __align__(16) T v[8];
+    __device__ __forceinline__ void load(const T* p, bool vec) {
+        if (vec) {
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-            reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+                reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f32(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f32(p[i]);
+            for (int i = 0; i < 8; ++i) v[i] = p[i];
+        }
     }
-}
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool vec, const float (&f)[8]) {
     __align__(16) T t[8];
@@ -84,10 +85,29 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArg
     constexpr int kHalf = kHd / 2;
     constexpr int kChunks = kHalf / 8;                 // threads of one head
     constexpr int kHeads = kAppendThreads / kChunks;   // heads taken at a time
+    constexpr int kBatch = sizeof(In) == 4 ? 2 : 3;
     pdl_launch_dependents();
-    pdl_wait();
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & 31;
+    const int nh = a.c.nh, nkv = a.c.nkv, all = nh + 2 * nkv;
+    const int d = (threadIdx.x % kChunks) * 8;
+    const int step = kHeads * static_cast<int>(gridDim.y);
+    int h0 = threadIdx.x / kChunks + static_cast<int>(blockIdx.y) * kHeads;
+    Eight<In> x0[kBatch], x1[kBatch];
+    auto load = [&]() {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int h = h0 + i * step;
+            if (h >= all) continue;
+            const In* src = h < nh ? static_cast<const In*>(a.q) + t * a.q_stride + h * kHd
+                            : h < nh + nkv ? static_cast<const In*>(a.k) + t * a.k_stride + (h - nh) * kHd
+                                           : static_cast<const In*>(a.v) + t * a.v_stride + (h - nh - nkv) * kHd;
+            x0[i].load(src + d, a.vec_in);
+            x1[i].load(src + d + kHalf, a.vec_in);
+        }
+    };
+    pdl_wait();
+    load();
     // the token's sequence: the number of sequences that end at or before it
     int seq = 0;
     for (int b0 = 0; b0 < a.c.num_seqs; b0 += 32) {
@@ -100,47 +120,55 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArg
         if (threadIdx.x == 0) record_error(a.c.status, DEV_BAD_INDEX);
         return;
     }
+    Eight<float> c0, c1, s0, s1;
+    c0.load(a.cos_t + pos * kHd + d, a.vec_table);
+    c1.load(a.cos_t + pos * kHd + d + kHalf, a.vec_table);
+    s0.load(a.sin_t + pos * kHd + d, a.vec_table);
+    s1.load(a.sin_t + pos * kHd + d + kHalf, a.vec_table);
     int64_t page = -1;
     const int64_t slot = pos >> a.c.page_shift;
     if (slot < a.c.max_pages) page = a.c.table[seq * a.c.max_pages + slot];
     const bool held = page >= 0 && page < a.c.num_pages;
     if (!held && threadIdx.x == 0) record_error(a.c.status, DEV_BAD_INDEX);
-    const int d = (threadIdx.x % kChunks) * 8;
-    float c0[8], c1[8], s0[8], s1[8];
-    load8(a.cos_t + pos * kHd + d, a.vec_table, c0);
-    load8(a.cos_t + pos * kHd + d + kHalf, a.vec_table, c1);
-    load8(a.sin_t + pos * kHd + d, a.vec_table, s0);
-    load8(a.sin_t + pos * kHd + d + kHalf, a.vec_table, s1);
-    const int nh = a.c.nh, nkv = a.c.nkv, all = held ? nh + 2 * nkv : nh;
     const int64_t in_page = (pos & ((1ll << a.c.page_shift) - 1)) * kHd + d;
-    for (int h = threadIdx.x / kChunks + static_cast<int>(blockIdx.y) * kHeads; h < all;
-         h += kHeads * static_cast<int>(gridDim.y)) {
-        const In* src = h < nh ? static_cast<const In*>(a.q) + t * a.q_stride + h * kHd
-                        : h < nh + nkv ? static_cast<const In*>(a.k) + t * a.k_stride + (h - nh) * kHd
-                                       : static_cast<const In*>(a.v) + t * a.v_stride + (h - nh - nkv) * kHd;
-        float x0[8], x1[8];
-        load8(src + d, a.vec_in, x0);
-        load8(src + d + kHalf, a.vec_in, x1);
-        if (h < nh + nkv) {
+    for (; h0 < all; h0 += kBatch * step) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float lo = __fsub_rn(__fmul_rn(x0[i], c0[i]), __fmul_rn(x1[i], s0[i]));
-                x1[i] = __fadd_rn(__fmul_rn(x1[i], c1[i]), __fmul_rn(x0[i], s1[i]));
-                x0[i] = lo;
+        for (int i = 0; i < kBatch; ++i) {
+            const int h = h0 + i * step;
+            if (h >= all || (h >= nh && !held)) continue;
+            float lo[8], hi[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                lo[e] = to_f32(x0[i].v[e]);
+                hi[e] = to_f32(x1[i].v[e]);
             }
+            if (h < nh + nkv) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float r = __fsub_rn(__fmul_rn(lo[e], c0.v[e]), __fmul_rn(hi[e], s0.v[e]));
+                    hi[e] = __fadd_rn(__fmul_rn(hi[e], c1.v[e]), __fmul_rn(lo[e], s1.v[e]));
+                    lo[e] = r;
+                }
+            }
+            Cache* dst;
+            bool vec = a.vec_cache;
+            if (h < nh) {
+                dst = static_cast<Cache*>(a.q_out) + (t * nh + h) * kHd + d;
+                vec = a.vec_qout;
+            } else {
+                const int hk = h < nh + nkv ? h - nh : h - nh - nkv;
+                dst = static_cast<Cache*>(h < nh + nkv ? a.kp : a.vp) + page * a.c.page_stride +
+                      (static_cast<int64_t>(hk) << a.c.page_shift) * kHd + in_page;
+            }
+            store8(dst, vec, lo);
+            store8(dst + kHalf, vec, hi);
         }
-        Cache* dst;
-        bool vec = a.vec_cache;
-        if (h < nh) {
-            dst = static_cast<Cache*>(a.q_out) + (t * nh + h) * kHd + d;
-            vec = a.vec_qout;
-        } else {
-            const int hk = h < nh + nkv ? h - nh : h - nh - nkv;
-            dst = static_cast<Cache*>(h < nh + nkv ? a.kp : a.vp) + page * a.c.page_stride +
-                  (static_cast<int64_t>(hk) << a.c.page_shift) * kHd + in_page;
+        if (h0 + kBatch * step < all) {
+            const int keep = h0;
+            h0 += kBatch * step;
+            load();
+            h0 = keep;
         }
-        store8(dst, vec, x0);
-        store8(dst + kHalf, vec, x1);
     }
 }
 
