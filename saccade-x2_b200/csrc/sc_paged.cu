@@ -35,7 +35,10 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 // heads in turn, so that the token's angles are loaded once for all of its heads; q, k and v heads
 // follow one another in the loop.  Bytes bound: q, k, v read, q' and the cache rows written, two
 // table rows per token.  The loads of the first heads do not depend on the token's place: they are issued before
-// it is looked up, and kBatch heads' loads are on their way at a time.
+// it is looked up.  16-bit rows hold the angles in registers and take two heads at a time (43 us at 2 x 2048 tokens
+// of 64 + 8 heads, bf16: 4.0 TB/s; from the L1 cache for each head 46 us); f32 rows, which need those registers,
+// take the angles from the cache (4.2 us at 1,200 tokens of 14 + 2 heads; held 5.8 us).  CTAs that stay and
+// fetch their next token beside the present one measured slower (50 us).
 constexpr int kAppendThreads = 256;
 
 struct AppendArgs {
@@ -80,12 +83,23 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&f)[8]) {
     }
 }
 
+__device__ __forceinline__ float4 load4(const float* p, bool vec) {
+    return vec ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+}
+// (x, y) by the angle of (c0, s0) in x and (c1, s1) in y, products and sums each rounded.
+__device__ __forceinline__ void rotate(float& x, float& y, float c0, float s0, float c1, float s1) {
+    const float r = __fsub_rn(__fmul_rn(x, c0), __fmul_rn(y, s0));
+    y = __fadd_rn(__fmul_rn(y, c1), __fmul_rn(x, s1));
+    x = r;
+}
+
 template <typename In, typename Cache, int kHd>
-__global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, sizeof(In) == 4 ? 4 : 3) k_paged_append(const AppendArgs a) {
     constexpr int kHalf = kHd / 2;
     constexpr int kChunks = kHalf / 8;                 // threads of one head
     constexpr int kHeads = kAppendThreads / kChunks;   // heads taken at a time
-    constexpr int kBatch = sizeof(In) == 4 ? 2 : 3;
+    constexpr bool kHeld = sizeof(In) == 2;            // the angles stay in registers
+    constexpr int kBatch = kHeld ? 2 : 1;
     pdl_launch_dependents();
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & 31;
@@ -120,11 +134,17 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArg
         if (threadIdx.x == 0) record_error(a.c.status, DEV_BAD_INDEX);
         return;
     }
-    Eight<float> c0, c1, s0, s1;
-    c0.load(a.cos_t + pos * kHd + d, a.vec_table);
-    c1.load(a.cos_t + pos * kHd + d + kHalf, a.vec_table);
-    s0.load(a.sin_t + pos * kHd + d, a.vec_table);
-    s1.load(a.sin_t + pos * kHd + d + kHalf, a.vec_table);
+    const float *ct = a.cos_t + pos * kHd + d, *st = a.sin_t + pos * kHd + d;
+    float4 angle[kHeld ? 8 : 1];
+    if constexpr (kHeld) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            angle[4 * q] = load4(ct + 4 * q, a.vec_table);
+            angle[4 * q + 1] = load4(st + 4 * q, a.vec_table);
+            angle[4 * q + 2] = load4(ct + kHalf + 4 * q, a.vec_table);
+            angle[4 * q + 3] = load4(st + kHalf + 4 * q, a.vec_table);
+        }
+    }
     int64_t page = -1;
     const int64_t slot = pos >> a.c.page_shift;
     if (slot < a.c.max_pages) page = a.c.table[seq * a.c.max_pages + slot];
@@ -144,10 +164,18 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendArg
             }
             if (h < nh + nkv) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float r = __fsub_rn(__fmul_rn(lo[e], c0.v[e]), __fmul_rn(hi[e], s0.v[e]));
-                    hi[e] = __fadd_rn(__fmul_rn(hi[e], c1.v[e]), __fmul_rn(lo[e], s1.v[e]));
-                    lo[e] = r;
+                for (int q = 0; q < 8; q += 4) {
+                    float4 c0, s0, c1, s1;
+                    if constexpr (kHeld) {
+                        c0 = angle[q], s0 = angle[q + 1], c1 = angle[q + 2], s1 = angle[q + 3];
+                    } else {
+                        c0 = load4(ct + q, a.vec_table), s0 = load4(st + q, a.vec_table);
+                        c1 = load4(ct + kHalf + q, a.vec_table), s1 = load4(st + kHalf + q, a.vec_table);
+                    }
+                    rotate(lo[q], hi[q], c0.x, s0.x, c1.x, s1.x);
+                    rotate(lo[q + 1], hi[q + 1], c0.y, s0.y, c1.y, s1.y);
+                    rotate(lo[q + 2], hi[q + 2], c0.z, s0.z, c1.z, s1.z);
+                    rotate(lo[q + 3], hi[q + 3], c0.w, s0.w, c1.w, s1.w);
                 }
             }
             Cache* dst;
