@@ -9,15 +9,15 @@ from .checkpoint import (SaccadeMlp, build_saccade_op, compile_mlp_checkpoint, e
                          load_mlp, load_saccade_checkpoint, read_safetensors, saccade_blocks,
                          write_safetensors)
 from .graph import CapturedStep
-from .logits import process_logits
+from .logits import LogitRules, process_logits
 from .compress import (ProfileRunner, compress_tensor_to_saccade, compute_percentile_threshold,
                        saccade_op_from_compressed)
 from .op import (GroupRouting, SaccadeConfig, SaccadeLinearGroup, SaccadeLinearOp, SparseDeltaMatrix, finalize,
                  is_c_tarq_bypassed, set_bypass_c_tarq, variance_heuristic)
-from .paged import paged_append, paged_attention
+from .paged import PagedKVCache, paged_append, paged_attention
 
 __all__ = [
-    "CapturedStep", "CTarqError", "GroupRouting", "LIB_PATH", "ProfileRunner", "SaccadeConfig", "SaccadeLinearGroup", "SaccadeLinearOp",
+    "CapturedStep", "CTarqError", "GroupRouting", "LIB_PATH", "LogitRules", "PagedKVCache", "ProfileRunner", "SaccadeConfig", "SaccadeLinearGroup", "SaccadeLinearOp",
     "SaccadeMlp", "SparseDeltaMatrix", "build_saccade_op", "compile_mlp_checkpoint", "compress_tensor_to_saccade",
     "compute_percentile_threshold", "extract_scalar_f32", "finalize", "is_c_tarq_bypassed", "load_mlp",
     "load_saccade_checkpoint", "paged_append", "paged_attention", "process_logits", "read_safetensors", "saccade_blocks", "saccade_op_from_compressed",

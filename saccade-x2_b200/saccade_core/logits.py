@@ -1,9 +1,14 @@
-"""process_logits: penalties for repeated tokens, biases and grammar masks on a step's logits, with the
+"""Logits processing:
+
+    process_logits   sc_qwen2_process_logits on tensors
+    LogitRules       the penalties, biases and masks of a batch of sequences, on the device
+
+Penalties for repeated tokens, biases and grammar masks on a step's logits, with the
 best token of each row (the argmax of saccade-runner/src/bin/verify.rs:98-130, which decodes without any
 of them)."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import Dict, Optional, Sequence, Union
 
 import torch
 
@@ -31,3 +36,74 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     mask r).  Ids are of the whole vocabulary throughout."""
     return _serve.process_logits(logits, history, prompt_len, hist_len, repetition, presence, frequency, bias_ptr, bias_ids,
                                  bias_vals, mask, mask_row, vocab_begin, out, return_best, status)
+
+
+class LogitRules:
+    """What a batch's logits go through: repetition, presence and frequency penalties (a number, or one per
+    sequence), bias (one {token: value} per sequence) and grammar masks (int32 [masks, words], one bit per
+    token; mask_row: each sequence's mask or -1).  The tensors stay where they are, so a captured step follows
+    what is written into them (a grammar's next mask, another penalty)."""
+
+    def __init__(self, batch: int, device, *, repetition: Union[None, float, Sequence[float]] = None,
+                 presence: Union[None, float, Sequence[float]] = None,
+                 frequency: Union[None, float, Sequence[float]] = None, bias: Optional[Sequence[Dict[int, float]]] = None,
+                 mask: Optional[torch.Tensor] = None, mask_row: Optional[Sequence[int]] = None):
+        def floats(v, what):
+            if v is None:
+                return None
+            t = torch.as_tensor(v, dtype=torch.float32)
+            if t.dim() == 0:
+                t = t.repeat(batch)
+            if t.shape != (batch,):
+                raise ValueError(f"{what} must be a number or one per sequence")
+            return t.to(device)
+
+        self.repetition = floats(repetition, "repetition")
+        if self.repetition is not None and not bool((self.repetition > 0).all()):
+            raise ValueError("a repetition penalty must be above 0")
+        self.presence, self.frequency = floats(presence, "presence"), floats(frequency, "frequency")
+        self.bias_ptr = self.bias_ids = self.bias_vals = None
+        if bias is not None:
+            if len(bias) != batch or max(map(len, bias), default=0) > 4095:
+                raise ValueError("bias must be one {token: value} per sequence, of at most 4095 tokens each")
+            ptr = [0]
+            for b in bias:
+                ptr.append(ptr[-1] + len(b))
+            self.bias_ptr = torch.tensor(ptr, dtype=torch.int32, device=device)
+            self.bias_ids = torch.tensor([t for b in bias for t in b], dtype=torch.int32, device=device)
+            self.bias_vals = torch.tensor([x for b in bias for x in b.values()], dtype=torch.float32, device=device)
+        self.mask = None if mask is None else mask.to(device)
+        self.mask_row = None if mask_row is None else torch.tensor(list(mask_row), dtype=torch.int32, device=device)
+
+    def apply(self, logits: torch.Tensor, *, rows: Optional[torch.Tensor] = None, history=None, prompt_len=None,
+              hist_len=None, vocab_begin: int = 0, out: Optional[torch.Tensor] = None,
+              status: Optional[torch.Tensor] = None):
+        """process_logits with these rules for all sequences, or for those of `rows` (a tensor of indices):
+        (logits, best ids, best values)."""
+        if rows is None:
+            pick = lambda t: t  # noqa: E731
+            bias = (self.bias_ptr, self.bias_ids, self.bias_vals)
+            mask_row = self.mask_row
+        else:
+            pick = lambda t: None if t is None else t[rows].contiguous()  # noqa: E731
+            bias, mask_row = self._bias_of(rows), pick(self.mask_row)
+            if self.mask is not None and mask_row is None:
+                mask_row = rows.to(device=self.mask.device, dtype=torch.int32)
+        return process_logits(logits, history=history, prompt_len=prompt_len, hist_len=hist_len,
+                              repetition=pick(self.repetition), presence=pick(self.presence),
+                              frequency=pick(self.frequency), bias_ptr=bias[0], bias_ids=bias[1], bias_vals=bias[2],
+                              mask=self.mask, mask_row=mask_row, vocab_begin=vocab_begin, out=out, return_best=True,
+                              status=status)
+
+    def _bias_of(self, rows: torch.Tensor):
+        """The bias entries of some sequences as a list of their own."""
+        if self.bias_ptr is None:
+            return None, None, None
+        ptr, idx = self.bias_ptr.tolist(), rows.tolist()
+        keep = [e for r in idx for e in range(ptr[r], ptr[r + 1])]
+        new = [0]
+        for r in idx:
+            new.append(new[-1] + ptr[r + 1] - ptr[r])
+        dev = self.bias_ids.device
+        take = torch.tensor(keep, dtype=torch.int64, device=dev)
+        return torch.tensor(new, dtype=torch.int32, device=dev), self.bias_ids[take], self.bias_vals[take]

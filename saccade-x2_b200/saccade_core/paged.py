@@ -2,8 +2,7 @@
 
     paged_append      sc_qwen2_paged_append: rotates q and k, writes k and v into the pages
     paged_attention   sc_qwen2_paged_attention: causal attention of every sequence's new tokens
-    PagePool          which pages are free (host side)
-    PagedKVCache      a model's pages, its pool and the block tables of its sequences
+    PagedKVCache      a model's pages of every layer, the free ones, and the block tables of its sequences
 
 The reference keeps one f32 cache tensor per sequence and concatenates to it (saccade-runner/src/
 model.rs:228-236).  Here a cache of f32, f16 or bf16 is cut into pages [kv heads][page][head dim] that
@@ -21,7 +20,7 @@ from typing import List, Optional
 import torch
 
 from . import _serve
-from ._lib import LIB, check
+from ._lib import LIB, SC_EDEVICE, SC_ETIMEOUT, CTarqError, check
 from .op import _DT
 
 
@@ -68,3 +67,73 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("out must be of the cache's type, or float16 from a float32 cache")
     return _serve.paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_len, max_q_len, max_kv_len, scale, out, code,
                                   return_lse, status)
+
+
+class PagedKVCache:
+    """Every layer's pages of a model, which of them are free, and the pages of up to max_seqs sequences.
+
+    k[layer], v[layer]: [pages, kv heads, page size, head dim]; a sequence (slot) has the same page
+    numbers in every layer.  block_table [max_seqs, pages of max_positions] and kv_len [max_seqs] live on
+    the device.  reserve() and release() run on the host and write the slot's row of the block table
+    on the current stream; the steps that read it are ordered behind them."""
+
+    def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, *, max_seqs: int,
+                 max_positions: int, dtype: torch.dtype = torch.float16, device="cuda:0"):
+        if layers < 1 or num_pages < 1 or max_seqs < 1 or max_positions < 1:
+            raise ValueError("a cache needs layers, pages, sequences and positions")
+        if page_size < 8 or page_size > 256 or page_size & (page_size - 1):
+            raise ValueError("page_size must be a power of two in 8..256")
+        if head_dim not in (64, 128):
+            raise ValueError("head_dim must be 64 or 128")
+        if dtype not in _DT:
+            raise ValueError("the cache must be float32, float16 or bfloat16")
+        self.page_size, self.num_pages, self.dtype = page_size, num_pages, dtype
+        self.max_seqs, self.max_positions, self.device = max_seqs, max_positions, torch.device(device)
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        self.k = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.block_table = torch.zeros(max_seqs, -(-max_positions // page_size), dtype=torch.int32, device=self.device)
+        self.kv_len = torch.zeros(max_seqs, dtype=torch.int32, device=self.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages: List[List[int]] = [[] for _ in range(max_seqs)]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def pages(self, slot: int) -> List[int]:
+        """The slot's pages, in order."""
+        return list(self._pages[slot])
+
+    def reserve(self, slot: int, positions: int) -> None:
+        """Gives the slot the pages that `positions` positions need (it keeps those it has); RuntimeError, and
+        nothing changed, where not enough are free."""
+        if positions < 0 or positions > self.max_positions:
+            raise ValueError(f"{positions} positions: the cache is made for up to {self.max_positions}")
+        have = self._pages[slot]
+        need = -(-positions // self.page_size) - len(have)
+        if need <= 0:
+            return
+        if need > len(self._free):
+            raise RuntimeError(f"{need} pages wanted, {len(self._free)} of {self.num_pages} free")
+        new = [self._free.pop() for _ in range(need)]
+        row = torch.tensor(new, dtype=torch.int32).pin_memory() if self.device.type == "cuda" else torch.tensor(
+            new, dtype=torch.int32)
+        self.block_table[slot, len(have):len(have) + need].copy_(row, non_blocking=True)
+        have.extend(new)
+
+    def release(self, slot: int) -> None:
+        """Takes the slot's pages back (what they hold stays until another sequence writes them)."""
+        self._free.extend(reversed(self._pages[slot]))
+        self._pages[slot] = []
+        self.kv_len[slot] = 0
+
+    def check_device(self) -> None:
+        """Raises where a kernel met a position, page or length outside the tables (or a wait ran out)."""
+        st = int(self.status.item())
+        if st:
+            self.status.zero_()
+            raise CTarqError(SC_ETIMEOUT if st == 1 else SC_EDEVICE,
+                             "a wait ran out in a paged-cache kernel" if st == 1 else
+                             "a position, page or length outside the paged cache's tables")

@@ -23,6 +23,11 @@ writes one f32 exchange buffer [y_base | y_delta | router sums] (sc_forward_spli
 summed over the group by one NCCL all-reduce, and sc_finalize_split routes every token on the
 summed sums and rounds.  The lm_head is vocab-parallel: each rank scores its slice of the
 vocabulary and greedy decoding all-gathers each rank's (max, argmax) per sequence.
+
+Serving (no reference counterpart: verify decodes one sequence greedily): a Qwen2Model on a PagedKVCache
+runs ragged batches (forward_paged: prompts in chunks beside decoding sequences, f32, f16 or bf16
+cache), and PagedDecoder decodes them with penalties, biases and grammar masks on the logits (LogitRules),
+each step one CUDA graph as GreedyDecoder's.
 """
 from __future__ import annotations
 
@@ -38,6 +43,8 @@ from . import _lib
 from ._lib import LIB, check
 from .compress import ProfileRunner, compress_tensor_to_saccade, compute_percentile_threshold
 from .graph import no_gc
+from .logits import LogitRules
+from .paged import PagedKVCache, paged_append, paged_attention
 from .op import GroupRouting, SaccadeConfig, SaccadeLinearGroup, SaccadeLinearOp, SparseDeltaMatrix, flush_deferred
 
 PROJ = ("q", "k", "v", "o", "gate", "up", "down")
@@ -181,10 +188,12 @@ def _u32(t):
 
 class Qwen2Model:
     """Qwen2Model::forward on one GPU, or one rank of a tensor-parallel group (tp = (rank, world,
-    process_group) with NCCL).  Serves up to `max_batch` sequences of up to `max_pos` positions."""
+    process_group) with NCCL).  Serves up to `max_batch` sequences of up to `max_pos` positions from a
+    contiguous f32 cache of its own (forward_tokens), or, given a PagedKVCache of this rank's KV heads
+    (paged_cache() makes one), that cache's sequences (forward_paged)."""
 
     def __init__(self, ck: Checkpoint, device=None, max_batch: int = 1, max_pos: int = 512, mode: str = "fast",
-                 tp=None, fused_route="none"):
+                 tp=None, fused_route="none", cache: Optional[PagedKVCache] = None):
         """fused_route: where a group of linears runs the 9..64-token launch, its router runs in the
         kernel that writes its input instead of a router launch of its own: "norm" for q,k,v and
         gate,up (the RMSNorm kernel), "all" also for down on one GPU (the SiLU * up kernel).  The
@@ -243,9 +252,17 @@ class Qwen2Model:
         cos, sin = rope_tables(cfg, max_pos)
         self.cos = torch.from_numpy(cos).to(dev)
         self.sin = torch.from_numpy(sin).to(dev)
-        shape = (max_batch, self.nkv, max_pos, hd)
-        self.k_cache = [torch.zeros(shape, dtype=torch.float32, device=dev) for _ in self.layers]
-        self.v_cache = [torch.zeros(shape, dtype=torch.float32, device=dev) for _ in self.layers]
+        self.cache = cache
+        if cache is not None:
+            want = (self.nkv, cache.page_size, hd)
+            if len(cache.k) != len(self.layers) or tuple(cache.k[0].shape[1:]) != want or cache.k[0].device != self.embed.device:
+                raise ValueError(f"the cache must hold {len(self.layers)} layers of pages {want} on {self.embed.device}")
+            if cache.max_positions > max_pos:
+                raise ValueError(f"the cache's {cache.max_positions} positions need max_pos of as many (the rotation tables)")
+        else:
+            shape = (max_batch, self.nkv, max_pos, hd)
+            self.k_cache = [torch.zeros(shape, dtype=torch.float32, device=dev) for _ in self.layers]
+            self.v_cache = [torch.zeros(shape, dtype=torch.float32, device=dev) for _ in self.layers]
         self.status = torch.zeros(4, dtype=torch.int32, device=dev)
         self._bufs = {}
         torch.backends.cuda.matmul.allow_fp16_reduced_precision_reduction = False
@@ -280,6 +297,46 @@ class Qwen2Model:
         """Runs T tokens (ids [T] int64, cache slot [T] and position [T] int32) through the model,
         appending their keys and values; returns the f32 logits [len(last), v1 - v0] of the tokens
         at indices `last` (int64) over this rank's vocabulary slice [v0, v1) (all of it on one GPU)."""
+        if self.cache is not None:
+            raise ValueError("a model on a paged cache runs forward_paged")
+        T, hd = ids.numel(), self.cfg.head_dim
+        scratch_bytes = int(LIB.sc_qwen2_attention_scratch(T, self.nh, self.nkv, hd, self.max_pos))
+        scratch = self._buf(("attn", T), (max(1, scratch_bytes // 4),), torch.float32)
+
+        def attend(li, q, k, v, a16, st):
+            check(LIB.sc_qwen2_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), self.cos.data_ptr(),
+                                           self.sin.data_ptr(), slot.data_ptr(), pos.data_ptr(), T, self.nh, self.nkv,
+                                           hd, self.max_pos, self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(),
+                                           st))
+            check(LIB.sc_qwen2_attention(q.data_ptr(), self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(),
+                                         slot.data_ptr(), pos.data_ptr(), T, self.nh, self.nkv, hd, self.max_pos,
+                                         max_query_pos, scratch.data_ptr(), scratch.numel() * 4, a16.data_ptr(), st))
+
+        return self._forward(ids, last, attend, torch.float16)
+
+    def forward_paged(self, ids: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+                      last: torch.Tensor, max_q_len: int, max_kv_len: int) -> torch.Tensor:
+        """Runs T tokens (ids [T] int64) of several sequences through the model on its paged cache: sequence b owns
+        rows cu_q[b]..cu_q[b + 1] and has kv_len[b] positions with them, in the pages of block_table[b] (reserved
+        by the caller).  Returns the f32 logits [len(last), v1 - v0] of the tokens at indices `last`.
+        max_q_len and max_kv_len bound the new tokens and positions of every sequence."""
+        c = self.cache
+        if c is None:
+            raise ValueError("forward_paged needs a model on a paged cache")
+        T, hd = ids.numel(), self.cfg.head_dim
+        qr = self._buf(("qr", T), (T, self.nh, hd), c.dtype)
+
+        def attend(li, q, k, v, a16, st):
+            paged_append(q.view(T, self.nh, hd), k.view(T, self.nkv, hd), v.view(T, self.nkv, hd), self.cos, self.sin,
+                         c.k[li], c.v[li], block_table, cu_q, kv_len, out=qr, status=c.status)
+            paged_attention(qr, c.k[li], c.v[li], block_table, cu_q, kv_len, max_q_len, max_kv_len,
+                            out=a16.view(T, self.nh, hd), status=c.status)
+
+        # the linears read f16 or bf16 (rounded to f16 as they read it); an f32 cache's attention writes f16
+        return self._forward(ids, last, attend, torch.bfloat16 if c.dtype == torch.bfloat16 else torch.float16)
+
+    def _forward(self, ids: torch.Tensor, last: torch.Tensor, attend, attn_dtype: torch.dtype) -> torch.Tensor:
+        """The layers around `attend(layer, q, k, v, out, stream)`, which rotates, appends and attends."""
         cfg, dev = self.cfg, self.device
         T = ids.numel()
         H, hd = cfg.hidden, cfg.head_dim
@@ -291,14 +348,12 @@ class Qwen2Model:
         q = self._buf(("q", T), (T, self.nh * hd), torch.float32)
         k = self._buf(("k", T), (T, self.nkv * hd), torch.float32)
         v = self._buf(("v", T), (T, self.nkv * hd), torch.float32)
-        a16 = self._buf(("a16", T), (T, self.nh * hd), torch.float16)
+        a16 = self._buf(("a16", T), (T, self.nh * hd), attn_dtype)
         delta = self._buf(("delta", T), (T, H), torch.float32)
         ni = self.i1 - self.i0
         g16 = self._buf(("g16", T), (T, ni), torch.float16)
         u16 = self._buf(("u16", T), (T, ni), torch.float16)
         m16 = self._buf(("m16", T), (T, ni), torch.float16)
-        scratch_bytes = int(LIB.sc_qwen2_attention_scratch(T, self.nh, self.nkv, hd, self.max_pos))
-        scratch = self._buf(("attn", T), (max(1, scratch_bytes // 4),), torch.float32)
         have_delta = False
         L0 = self.layers[0]
         fuse_norm = self.fused_route in ("norm", "all")
@@ -318,13 +373,7 @@ class Qwen2Model:
                 check(LIB.sc_qwen2_add_rmsnorm(resid.data_ptr(), dptr, L["norm_in"].data_ptr(), T, H, eps,
                                                x16.data_ptr(), _lib.SC_F16, st))
                 L["qkv"].forward(x16, out_dtype=torch.float32, outs=[q, k, v], biases=L["bias"])
-            check(LIB.sc_qwen2_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), self.cos.data_ptr(),
-                                           self.sin.data_ptr(), slot.data_ptr(), pos.data_ptr(), T, self.nh, self.nkv,
-                                           hd, self.max_pos, self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(),
-                                           st))
-            check(LIB.sc_qwen2_attention(q.data_ptr(), self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(),
-                                         slot.data_ptr(), pos.data_ptr(), T, self.nh, self.nkv, hd, self.max_pos,
-                                         max_query_pos, scratch.data_ptr(), scratch.numel() * 4, a16.data_ptr(), st))
+            attend(li, q, k, v, a16, st)
             self._row_layer(L["o"], a16, delta, ("o", T))
             if r_gu is not None:
                 check(LIB.sc_qwen2_add_rmsnorm_route(resid.data_ptr(), delta.data_ptr(), L["norm_post"].data_ptr(), T,
@@ -375,6 +424,15 @@ class Qwen2Model:
         hilo[nl:].copy_((xn - hi.float()).to(torch.float16))
         p = torch.mm(hilo, self.lm_head_t, out_dtype=torch.float32)
         return p[:nl] + p[nl:]
+
+    @staticmethod
+    def paged_cache(ck: Checkpoint, num_pages: int, *, max_seqs: int, max_positions: int, page_size: int = 64,
+                    dtype: torch.dtype = torch.float16, device=None, tp=None) -> PagedKVCache:
+        """A paged cache for a model of this checkpoint (a tensor-parallel rank's KV heads)."""
+        rank, world = (0, 1) if tp is None else tp[:2]
+        _, _, k0, k1 = head_split(ck.cfg, rank, world)
+        return PagedKVCache(len(ck.blocks), num_pages, page_size, k1 - k0, ck.cfg.head_dim, max_seqs=max_seqs,
+                            max_positions=max_positions, dtype=dtype, device=ck.embed.device if device is None else device)
 
     def undecided_routes(self) -> int:
         """Row-layer tokens routed on the f64 score inside the f32 error bound (tensor parallel only)."""
@@ -439,6 +497,17 @@ def prefill_indices(prompt: torch.Tensor):
     return ids, slot, pos
 
 
+def best_of_ranks(m: Qwen2Model, val: torch.Tensor, idx: torch.Tensor, out: torch.Tensor, cand: torch.Tensor,
+                  gath: torch.Tensor) -> torch.Tensor:
+    """The first of the ranks' maxima (val, global idx [n]) into out; cand [n, 2] and gath [world, n, 2] f32 buffers."""
+    cand[:, 0].copy_(val)
+    cand[:, 1].copy_(idx)  # ids < 2^24 are exact in f32
+    torch.distributed.all_gather_into_tensor(gath, cand, group=m.group)
+    best = torch.argmax(gath[:, :, 0], dim=0)  # first rank holding the maximum
+    out.copy_(gath[:, :, 1].gather(0, best[None, :])[0].to(torch.int64))
+    return out
+
+
 class GreedyDecoder:
     """Prefill, then greedy decoding one token per sequence per step (verify.rs:98-130), each decode
     step replayed as one CUDA graph: token ids in, argmax token ids out (the step also copies them
@@ -468,14 +537,8 @@ class GreedyDecoder:
         if n not in self._xchg:
             self._xchg[n] = (torch.zeros(n, 2, dtype=torch.float32, device=m.device),
                              torch.zeros(m.world, n, 2, dtype=torch.float32, device=m.device))
-        cand, gath = self._xchg[n]
         val, idx = torch.max(logits, dim=-1)
-        cand[:, 0].copy_(val)
-        cand[:, 1].copy_(idx + m.v0)  # ids < 2^24 are exact in f32
-        torch.distributed.all_gather_into_tensor(gath, cand, group=m.group)
-        best = torch.argmax(gath[:, :, 0], dim=0)  # first rank holding the maximum
-        out.copy_(gath[:, :, 1].gather(0, best[None, :])[0].to(torch.int64))
-        return out
+        return best_of_ranks(m, val, idx + m.v0, out, *self._xchg[n])
 
     def prefill(self, prompt: torch.Tensor, chunk: int = 0) -> torch.Tensor:
         """Runs the prompts [B, S] (`chunk` sequences per pass, all at once by default) and returns the
@@ -558,3 +621,157 @@ class GreedyDecoder:
                 gaps.append((top[:, 0] - top[:, 1]).cpu())
         toks = torch.stack(out, dim=1)
         return (toks, torch.stack(gaps, dim=1)) if record_logits else toks
+
+
+class PagedDecoder:
+    """Decodes a batch of ragged prompts on a model's paged cache, with LogitRules on every step's logits.
+
+    start() takes the prompts, reserves the pages of their tokens and runs them in passes of at most `chunk`
+    tokens per sequence (long prompts in several passes, shorter ones beside them); step() decodes one
+    token of every sequence, as a replay of one captured graph after capture().  The decoder owns the cache's
+    slots 0 .. batch - 1 while it runs; finish() gives their pages back."""
+
+    def __init__(self, model: Qwen2Model, batch: int, rules: Optional[LogitRules] = None):
+        if model.cache is None:
+            raise ValueError("PagedDecoder needs a model on a paged cache")
+        c, dev = model.cache, model.device
+        if batch < 1 or batch > c.max_seqs:
+            raise ValueError(f"batch must be 1..{c.max_seqs} (the cache's sequences)")
+        self.model, self.B, self.cache, self.rules = model, batch, c, rules or LogitRules(batch, dev)
+        self.ids = torch.zeros(batch, dtype=torch.int64, device=dev)
+        self.history = torch.zeros(batch, c.max_positions + 1, dtype=torch.int32, device=dev)
+        self.hist_len = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.prompt_len = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.cu_q = torch.arange(batch + 1, dtype=torch.int32, device=dev)
+        self.last = torch.arange(batch, dtype=torch.int64, device=dev)
+        self.table, self.kv_len = c.block_table[:batch], c.kv_len[:batch]
+        self.raw = self.logits = None           # the last step's logits before and after the rules
+        self.lengths = [0] * batch              # positions held, on the host
+        self.graph = None
+        self.stream = torch.cuda.Stream(device=dev)
+        self._xchg = (torch.zeros(batch, 2, dtype=torch.float32, device=dev),
+                      torch.zeros(model.world, batch, 2, dtype=torch.float32, device=dev)) if model.world > 1 else None
+
+    def _choose(self, logits: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The rules applied to a step's logits of all sequences (or of `rows`), and the next tokens."""
+        m, pick = self.model, (lambda t: t) if rows is None else (lambda t: t[rows].contiguous())
+        out, best, value = self.rules.apply(
+            logits, rows=rows, history=pick(self.history), prompt_len=pick(self.prompt_len),
+            hist_len=pick(self.hist_len), vocab_begin=m.v0, status=self.cache.status)
+        if m.world > 1:
+            n = best.shape[0]
+            best = best_of_ranks(m, value, best, best, self._xchg[0][:n], self._xchg[1][:, :n].contiguous())
+        self.raw, self.logits = logits, out
+        return best
+
+    def _take(self, rows: torch.Tensor, tokens: torch.Tensor) -> None:
+        """The chosen tokens of sequences `rows` become their history's last and the next step's input."""
+        at = self.hist_len[rows].long()
+        self.history[rows, at] = tokens.to(torch.int32)
+        self.hist_len[rows] += 1
+        self.ids[rows] = tokens
+
+    def start(self, prompts, chunk: int = 2048) -> torch.Tensor:
+        """Runs the prompts (a list of `batch` 1-D id tensors, each of at least one token) and returns the first
+        tokens [batch]."""
+        m, c, dev = self.model, self.cache, self.model.device
+        if len(prompts) != self.B or any(p.dim() != 1 or p.numel() < 1 for p in prompts):
+            raise ValueError(f"{self.B} prompts of at least one token are wanted")
+        if chunk < 1:
+            raise ValueError("chunk must be at least 1")
+        lens = [int(p.numel()) for p in prompts]
+        if max(lens) > c.max_positions:
+            raise ValueError(f"a prompt of {max(lens)} tokens: the cache is made for up to {c.max_positions}")
+        with torch.cuda.device(dev), torch.cuda.stream(self.stream):
+            for b, n in enumerate(lens):
+                c.reserve(b, n)
+                self.history[b, :n] = prompts[b].to(dev, torch.int32)
+            self.prompt_len.copy_(torch.tensor(lens, dtype=torch.int32))
+            self.hist_len.copy_(self.prompt_len)
+            done = [0] * self.B
+            while True:
+                part = [(b, done[b], min(lens[b], done[b] + chunk)) for b in range(self.B) if done[b] < lens[b]]
+                if not part:
+                    break
+                ids = torch.cat([prompts[b][i:j].to(dev, torch.int64) for b, i, j in part])
+                cu = [0]
+                for _, i, j in part:
+                    cu.append(cu[-1] + j - i)
+                slots = torch.tensor([b for b, _, _ in part], device=dev)
+                ends = [n for n, (b, _, j) in enumerate(part) if j == lens[b]]  # the prompts that end in this pass
+                kv = torch.tensor([j for _, _, j in part], dtype=torch.int32, device=dev)
+                last = torch.tensor([cu[n + 1] - 1 for n in (ends or [0])], device=dev)
+                logits = m.forward_paged(ids, c.block_table[slots], torch.tensor(cu, dtype=torch.int32, device=dev), kv, last,
+                                         max(j - i for _, i, j in part), max(j for _, _, j in part))
+                if ends:
+                    rows = slots[torch.tensor(ends, device=dev)]
+                    self._take(rows, self._choose(logits, rows))
+                for b, _, j in part:
+                    done[b] = j
+            self.kv_len.copy_(self.prompt_len)
+            self.lengths = lens
+            first = self.ids.clone()
+        self.stream.synchronize()
+        return first
+
+    def _step(self) -> None:
+        self.kv_len.add_(1)
+        logits = self.model.forward_paged(self.ids, self.table, self.cu_q, self.kv_len, self.last, 1,
+                                          self.cache.max_positions)
+        self._take(self.last, self._choose(logits))
+
+    def _reserve_next(self) -> None:
+        if max(self.lengths) >= self.cache.max_positions:
+            raise RuntimeError(f"a sequence has all of the cache's {self.cache.max_positions} positions")
+        for b in range(self.B):
+            self.cache.reserve(b, self.lengths[b] + 1)
+
+    def capture(self) -> None:
+        """Records a step as a CUDA graph, after one eager step that sizes its buffers; that step counts (it
+        decodes a token)."""
+        with torch.cuda.device(self.model.device), torch.cuda.stream(self.stream):
+            self._reserve_next()
+            self._step()
+            self.lengths = [n + 1 for n in self.lengths]
+        self.stream.synchronize()
+        eager = self.raw, self.logits
+        self.graph = torch.cuda.CUDAGraph()
+        with no_gc(), torch.cuda.graph(self.graph, stream=self.stream):
+            self._step()
+        self._graph_logits = self.raw, self.logits  # written by every replay
+        self.raw, self.logits = eager
+        self.stream.synchronize()
+        flush_deferred()
+
+    def step(self) -> torch.Tensor:
+        """One decode step on the decoder's stream: the sequences' next tokens [batch] (device)."""
+        with torch.cuda.device(self.model.device), torch.cuda.stream(self.stream):
+            self._reserve_next()
+            if self.graph is not None:
+                self.graph.replay()
+                self.raw, self.logits = self._graph_logits
+            else:
+                self._step()
+            self.lengths = [n + 1 for n in self.lengths]
+        return self.ids
+
+    def generate(self, prompts, steps: int, *, chunk: int = 2048, graph: bool = True) -> torch.Tensor:
+        """Tokens [batch, steps] after the prompts."""
+        self.stream.wait_stream(torch.cuda.current_stream(self.model.device))
+        out = [self.start(prompts, chunk)]
+        if graph and self.graph is None and steps > 1:
+            self.capture()
+            out.append(self.ids.clone())
+        while len(out) < steps:
+            self.step()
+            self.stream.synchronize()
+            out.append(self.ids.clone())
+        torch.cuda.current_stream(self.model.device).wait_stream(self.stream)
+        return torch.stack(out[:steps], dim=1)
+
+    def finish(self) -> None:
+        """Gives the sequences' pages back, after the steps in flight."""
+        self.stream.synchronize()
+        for b in range(self.B):
+            self.cache.release(b)
+        self.lengths = [0] * self.B
