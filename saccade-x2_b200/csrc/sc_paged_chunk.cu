@@ -202,22 +202,25 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
         bool ok = true;
         const PagedRow mine(half * 128 + row, 128, G);
         PagedJoin join{0, 0, 0, 0, 0};
-        while (ok && w.next(kv, A.max_q, tt, C::kKeys)) {
+        PagedWalk wn = w;
+        bool more = wn.next(kv, A.max_q, tt, C::kKeys);
+        while (ok && more) {
+            w = wn;
             const int n = w.t1 - w.t0;
             const bool two = w.rt * tt + per < w.s.q_len;
             if (!w.whole() && w.t0 == 0)
-                join = PagedJoin{w.s.row0, w.s.q_len, w.h, w.rt,
-                                 static_cast<int>((w.at - n + w.tiles - 1) / cut.per) - static_cast<int>(blockIdx.x) + 1};
+                join = PagedJoin{w.s.row0, w.s.q_len, w.h, w.rt, w.pieces(cut)};
             if (half == 1 && !two) {
                 it += 2 * n;
                 // a cut item's second half is empty: its rows are never joined
+                more = wn.next(kv, A.max_q, tt, C::kKeys);
                 continue;
             }
             const int tok = mine.token(w.rt, tt, w.s.q_len);
             const int start = w.s.kv_len - w.s.q_len;
-            const int pos = tok >= 0 ? start + tok : -1;
             const int first_pos = start + w.rt * tt + half * per;  // the least position of the half's rows
             const int keys = start + min((w.rt + 1) * tt, w.s.q_len);
+            const int pos = tok >= 0 ? start + tok : keys - 1;  // (a row of no token: as little masked as any)
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < n; ++j, ++count) {
                 const int k0 = (w.t0 + j) * C::kKeys;
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                 const bool edge = k0 + C::kKeys > first_pos + 1;
                 const int lim = pos - k0;  // columns up to it are attended
                 auto mask = [&](uint32_t* v, int c) {
-                    if (edge) {
+                    if (edge && !__all_sync(0xffffffffu, lim >= 32 * c + 31)) {
                         const int x = lim - 32 * c;
                         const uint32_t live = x >= 31 ? 0xFFFFFFFFu : x < 0 ? 0u : (2u << x) - 1u;
 #pragma unroll
@@ -315,6 +318,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                 if (lane == 0) mbar_arrive(&p_full[half]);
             }
             it += 2 * n;
+            more = wn.next(kv, A.max_q, tt, C::kKeys);  // while the last product ends
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&o_full[half], items & 1, kv.status));
             ++items;
             if (!ok) break;

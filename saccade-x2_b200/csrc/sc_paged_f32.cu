@@ -275,8 +275,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
             }
         }
         if (!whole && w.t0 == 0)
-            join = PagedJoin{w.s.row0, w.s.q_len, w.h, w.rt,
-                             static_cast<int>((w.at - (w.t1 - w.t0) + w.tiles - 1) / cut.per) - static_cast<int>(blockIdx.x) + 1};
+            join = PagedJoin{w.s.row0, w.s.q_len, w.h, w.rt, w.pieces(cut)};
     }
     if (tid == 0) A.sc.join[blockIdx.x] = join;
 }
