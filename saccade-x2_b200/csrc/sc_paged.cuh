@@ -62,7 +62,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedKv& p, int b, int64_t m
 // items, sequences first, then KV heads, then row tiles, form one line that is cut into equal pieces,
 // one per CTA: no CTA has more than one tile above the mean whatever the lengths are.  Before its tiles an item
 // has one more unit on the line, for what it costs besides them (queries, output): without it the CTAs
-// with many short items are the last (attend 16 prompts of 129..512 tokens: 77 us, with it 67).  An item cut by a
+// with many short items are the last (16 prompts of 129..512 tokens: 81 us, with it 71).  An item cut by a
 // piece's border leaves partial results (unnormalised output, maximum, sum) in the scratch, one slot
 // for the item that the CTA continues (0) and one for the item that it begins and does not finish (1);
 // k_paged_combine joins them in order.

@@ -74,38 +74,57 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
         const int start = w.s.kv_len - w.s.q_len;
         const int keys = start + min((w.rt + 1) * tt, w.s.q_len);
         const int32_t* table = kv.table + w.b * kv.max_pages;
-        auto load = [&](const void* pages, float* dst, int t) {  // a K or V tile, asynchronously
-            const uint32_t d0 = smem_u32(dst);
-            for (int i = tid; i < C::kKeys * (kHd / 4); i += C::kThreads) {
-                const int r = i / (kHd / 4), c = i % (kHd / 4), key = t * C::kKeys + r;
-                const float* src = static_cast<const float*>(pages);
-                bool ok = key < keys;
-                if (ok) {
-                    const int64_t page = table[key >> kv.page_shift];
-                    ok = page >= 0 && page < kv.num_pages;
-                    if (ok)
-                        src += page * kv.page_stride +
-                               ((static_cast<int64_t>(w.h) << kv.page_shift) + (key & ((1 << kv.page_shift) - 1))) * kHd + c * 4;
-                    else
-                        record_error(kv.status, DEV_BAD_INDEX);
-                }
-                cp16(d0 + (r * C::kLd + c * 4) * 4, src, ok);
+        // this thread copies chunk `cc` of rows cr + kStep j: their places in the pages are found for a K tile and
+        // kept for its V tile
+        constexpr int kStep = C::kThreads / (kHd / 4), kCopies = C::kKeys / kStep;
+        const int cr = tid / (kHd / 4), cc = tid % (kHd / 4) * 4;
+        int64_t place[kCopies];
+        int id[kCopies];
+        auto look_up = [&](int t) {  // the rows' pages, a tile ahead
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                const int key = t * C::kKeys + cr + kStep * j;
+                id[j] = key < keys ? table[key >> kv.page_shift] : -1;
             }
+        };
+        auto find = [&](int t) {
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                const int key = t * C::kKeys + cr + kStep * j;
+                if (id[j] >= 0 && id[j] < kv.num_pages) {
+                    place[j] = id[j] * kv.page_stride +
+                               ((static_cast<int64_t>(w.h) << kv.page_shift) + (key & ((1 << kv.page_shift) - 1))) * kHd + cc;
+                } else {
+                    if (key < keys) record_error(kv.status, DEV_BAD_INDEX);
+                    place[j] = -1;  // zeros
+                }
+            }
+        };
+        auto load = [&](const void* pages, float* dst) {  // a K or V tile, asynchronously
+            const uint32_t d0 = smem_u32(dst + cr * C::kLd + cc);
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j)
+                cp16(d0 + j * kStep * C::kLd * 4, static_cast<const float*>(pages) + (place[j] < 0 ? 0 : place[j]), place[j] >= 0);
             cp_commit();
         };
-        __syncthreads();  // the item before has read its tiles
-        load(kv.k, sk, w.t0);
-        load(kv.v, sv, w.t0);
-        for (int i = tid; i < kRows * (kHd / 4); i += C::kThreads) {
-            const int r = i / (kHd / 4), c = i % (kHd / 4);
-            const PagedRow row(r, kRows, G);
+        look_up(w.t0);
+        constexpr int kQueries = kRows * (kHd / 4) / C::kThreads;
+        float4 qv[kQueries];
+#pragma unroll
+        for (int j = 0; j < kQueries; ++j) {  // the query rows this thread stages
+            const PagedRow row(cr + kStep * j, kRows, G);
             const int tok = row.token(w.rt, tt, w.s.q_len);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            qv[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (tok >= 0)
-                v = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + (w.s.row0 + tok) * A.q_stride +
-                                                     (w.h * G + row.g) * kHd + c * 4);
-            *reinterpret_cast<float4*>(sq + r * C::kLd + c * 4) = v;
+                qv[j] = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + (w.s.row0 + tok) * A.q_stride +
+                                                         (w.h * G + row.g) * kHd + cc);
         }
+        find(w.t0);
+        __syncthreads();  // the item before has read its tiles
+        load(kv.k, sk);
+        load(kv.v, sv);
+#pragma unroll
+        for (int j = 0; j < kQueries; ++j) *reinterpret_cast<float4*>(sq + (cr + kStep * j) * C::kLd + cc) = qv[j];
         int pos[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -122,6 +141,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
             for (int c = 0; c < kC8 / 2; ++c) o[i][c] = 0;
         }
         for (int t = w.t0; t < w.t1; ++t) {
+            if (t + 1 < w.t1) look_up(t + 1);
             cp_wait<1>();
             __syncthreads();  // K(t) is there (and the queries)
             uint64_t s2[4][C::kKpt];
@@ -147,8 +167,12 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                     }
             }
             __syncthreads();  // K(t) has been read
-            if (t + 1 < w.t1) load(kv.k, sk, t + 1);
-            else cp_commit();
+            if (t + 1 < w.t1) {
+                find(t + 1);
+                load(kv.k, sk);
+            } else {
+                cp_commit();
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float s[C::kKpt], mx = -INFINITY;
@@ -200,7 +224,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                 }
             }
             __syncthreads();  // V(t) and the weights have been read
-            if (t + 1 < w.t1) load(kv.v, sv, t + 1);
+            if (t + 1 < w.t1) load(kv.v, sv);
             else cp_commit();
         }
         cp_wait<0>();
