@@ -126,18 +126,19 @@ SC_API sc_status sc_qwen2_paged_append(const void* q, const void* k, const void*
                                        int64_t max_pages, const int32_t* cu_q, const int32_t* kv_len, int64_t num_seqs,
                                        void* q_out, uint32_t* status, void* stream);
 
-/* Scratch bytes sc_qwen2_paged_attention needs (no initial contents; one call uses it at a time). */
-SC_API size_t sc_qwen2_paged_attention_scratch(int64_t tokens, int64_t num_seqs, int num_heads, int num_kv_heads,
-                                               int head_dim, int64_t max_q_len, int cache_dtype);
+/* Scratch bytes sc_qwen2_paged_attention needs with these arguments (no initial contents; one call uses it at
+ * a time); 0 for short sequences of few new tokens, and for arguments it refuses. */
+SC_API size_t sc_qwen2_paged_attention_scratch(int64_t num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                               int64_t max_q_len, int64_t max_kv_len, int cache_dtype);
 
 /* Causal attention of each sequence's new tokens over its pages: the token at position p attends
  * positions 0..p, o = sum softmax(scale * q . k) v per query head (grouped onto the KV heads), f32
  * sums and softmax statistics.  q [tokens][num_heads][head_dim] of cache_dtype, rows q_stride elements
  * apart; out [tokens][num_heads][head_dim] contiguous, out_dtype = cache_dtype (an f32 cache may also
  * write SC_F16, the linears' input).  lse (nullable, f32 [tokens][num_heads]) = log sum exp(scale * q . k).
- * A token at a negative position attends nothing: its output is 0, its lse -inf.  max_q_len bounds
- * every sequence's new tokens (one sequence beyond it is skipped and recorded); max_kv_len is the
- * cached positions' bound.  16-bit caches need q, the pages and their strides 16-byte aligned and run
+ * A token at a negative position attends nothing: its output is 0, its lse -inf.  max_q_len and max_kv_len bound
+ * every sequence's new tokens and positions and choose the kernels (a sequence with more new tokens is skipped and
+ * recorded; more positions are attended all the same).  16-bit caches need q, the pages and their strides 16-byte aligned and run
  * on the tensor cores; cached values at covered positions must be finite. */
 SC_API sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                                           int cache_dtype, int64_t num_pages, int64_t page_stride, int page_size,

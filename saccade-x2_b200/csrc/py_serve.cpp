@@ -231,8 +231,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (want_lse) lse = at::empty({tokens, nh}, opt.dtype(at::kFloat));
         if (tokens > 0 && c.seqs > 0) {
             if (max_q > tokens) max_q = tokens;
-            const size_t bytes = f_attention_scratch(tokens, c.seqs, static_cast<int>(nh), static_cast<int>(c.nkv),
-                                                     static_cast<int>(c.hd), max_q, c.dtype);
+            const size_t bytes = f_attention_scratch(c.seqs, static_cast<int>(nh), static_cast<int>(c.nkv),
+                                                     static_cast<int>(c.hd), max_q, max_kv, c.dtype);
             const c10::DataPtr ws = scratch(bytes);
             if (!passed(f_attention(q.data_ptr(), qs, c.k, c.v, c.dtype, c.pages, c.stride, static_cast<int>(c.page), c.table,
                                     c.max_pages, c.cu_q, c.kv_len, c.seqs, tokens, static_cast<int>(nh),

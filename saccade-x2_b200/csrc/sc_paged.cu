@@ -269,17 +269,36 @@ int sm_count() {
 // The kernel of a call and its work division.
 struct PagedPlan {
     enum Kind { kF32, kDecode, kChunk } kind;
-    int ctas;
+    int64_t ctas;
     PagedTiling tl;
+    int cluster;     // CTAs of an item's cluster; 0: the line of key tiles is cut, the pieces joined through the scratch
+    size_t scratch;
 };
-static PagedPlan paged_plan(int dtype, int nh, int nkv, int hd, int64_t max_q) {
-    const int G = nh / nkv;
+static PagedPlan paged_plan(int dtype, int64_t num_seqs, int nh, int nkv, int hd, int64_t max_q, int64_t max_kv) {
+    const int G = nh / nkv, sms = sm_count();
+    const bool few = max_q * G <= 16;
+    PagedPlan p{};
     if (dtype == SC_F32) {
-        if (max_q * G <= 16) return {PagedPlan::kF32, 2 * sm_count(), {16, 16, 16 / G, 64}};
-        return {PagedPlan::kF32, hd == 64 ? 2 * sm_count() : sm_count(), {64, 64, 64 / G, 64}};
+        p.kind = PagedPlan::kF32;
+        p.ctas = few || hd == 64 ? 2 * sms : sms;
+        p.tl = few ? PagedTiling{16, 16, 16 / G, 64} : PagedTiling{64, 64, 64 / G, 64};
+    } else if (few) {
+        p.kind = PagedPlan::kDecode;
+        p.ctas = 2 * sms;
+        p.tl = {16, 16, 16 / G, 64};
+        if (max_kv <= kClusterKeys) {
+            const int64_t items = num_seqs * nkv;
+            p.cluster = 1;
+            while (p.cluster < 8 && items * p.cluster * 2 <= p.ctas && p.cluster * 2 * p.tl.kt <= max_kv) p.cluster *= 2;
+            p.ctas = items * p.cluster;
+        }
+    } else {
+        p.kind = PagedPlan::kChunk;
+        p.ctas = sms;
+        p.tl = {256, 128, 2 * (128 / G), 128};
     }
-    if (max_q * G <= 16) return {PagedPlan::kDecode, 2 * sm_count(), {16, 16, 16 / G, 64}};
-    return {PagedPlan::kChunk, sm_count(), {256, 128, 2 * (128 / G), 128}};
+    if (p.cluster == 0) p.scratch = paged_scratch_bytes(p.ctas, p.tl.rows, hd);
+    return p;
 }
 
 static int64_t elem_size(int dtype) { return dtype == SC_F32 ? 4 : 2; }
@@ -385,14 +404,12 @@ sc_status sc_qwen2_paged_append(const void* q, const void* k, const void* v, int
     return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
 }
 
-size_t sc_qwen2_paged_attention_scratch(int64_t tokens, int64_t num_seqs, int num_heads, int num_kv_heads, int head_dim,
-                                        int64_t max_q_len, int cache_dtype) {
-    (void)tokens, (void)num_seqs;
-    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_heads / num_kv_heads > kPagedMaxGroup ||
-        max_q_len <= 0)
+size_t sc_qwen2_paged_attention_scratch(int64_t num_seqs, int num_heads, int num_kv_heads, int head_dim, int64_t max_q_len,
+                                        int64_t max_kv_len, int cache_dtype) {
+    if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads ||
+        num_heads / num_kv_heads > kPagedMaxGroup || max_q_len <= 0 || max_kv_len <= 0 || (head_dim != 64 && head_dim != 128))
         return 0;
-    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, head_dim, max_q_len);
-    return paged_scratch_bytes(p.ctas, p.tl.rows, head_dim);
+    return paged_plan(cache_dtype, num_seqs, num_heads, num_kv_heads, head_dim, max_q_len, max_kv_len).scratch;
 }
 
 sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
@@ -419,20 +436,21 @@ sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* 
     if (!aligned16(q) || (tokens > 1 && q_stride * cs % 16) || !aligned16(k_pages) || !aligned16(v_pages) ||
         page_stride * cs % 16 || !aligned16(out))
         return paged_bad(who, "q, the pages, their strides and out must be 16-byte aligned");
-    if (scratch_bytes < sc_qwen2_paged_attention_scratch(tokens, num_seqs, num_heads, num_kv_heads, head_dim, max_q_len,
-                                                         cache_dtype)) {
+    const PagedPlan p = paged_plan(cache_dtype, num_seqs, num_heads, num_kv_heads, head_dim, max_q_len, max_kv_len);
+    if (scratch_bytes < p.scratch) {
         set_error(std::string(who) + ": scratch too small");
         return SC_ENOMEM;
     }
+    if (p.scratch > 0 && (!scratch || !aligned16(scratch))) return paged_bad(who, "scratch must be 16-byte aligned");
+    if (p.ctas > 0x7fffffff) return paged_bad(who, "too many sequences");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (!scratch || !aligned16(scratch)) return paged_bad(who, "scratch must be 16-byte aligned");
-    const PagedPlan p = paged_plan(cache_dtype, num_heads, num_kv_heads, head_dim, max_q_len);
+    const int ctas = static_cast<int>(p.ctas);
     const PagedLaunch a{c, q, q_stride, max_q_len, {out, lse, scale * 1.4426950408889634f}, p.tl,
-                        paged_scratch(scratch, p.ctas, p.tl.rows, head_dim)};
-    cudaError_t e = p.kind == PagedPlan::kF32      ? launch_paged_f32(a, out_dtype, head_dim, p.ctas, s)
-                    : p.kind == PagedPlan::kDecode ? launch_paged_decode(a, cache_dtype, head_dim, p.ctas, s)
-                                                   : launch_paged_chunk(a, cache_dtype, head_dim, p.ctas, s);
-    if (e == cudaSuccess) e = launch_paged_combine(a, out_dtype, head_dim, p.ctas, s);
+                        paged_scratch(scratch, p.cluster ? 0 : p.ctas, p.tl.rows, head_dim)};
+    cudaError_t e = p.kind == PagedPlan::kF32      ? launch_paged_f32(a, out_dtype, head_dim, ctas, s)
+                    : p.kind == PagedPlan::kDecode ? launch_paged_decode(a, cache_dtype, head_dim, ctas, p.cluster, s)
+                                                   : launch_paged_chunk(a, cache_dtype, head_dim, ctas, s);
+    if (e == cudaSuccess && p.cluster == 0) e = launch_paged_combine(a, out_dtype, head_dim, ctas, s);
     return e == cudaSuccess ? SC_OK : cuda_fail(e, who);
 }
 

@@ -13,6 +13,7 @@
 
 namespace sc {
 
+constexpr int64_t kClusterKeys = 2048;  // positions up to which few new tokens go to clusters
 constexpr int kPagedMaxGroup = 64;     // query heads per KV head
 constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
 
@@ -342,7 +343,8 @@ cudaError_t paged_allow_smem(Kern kern, std::atomic<uint64_t>& flags, int bytes)
     return e;
 }
 
-cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
+// cluster 0: the line cut into `ctas` pieces; otherwise ctas = items * cluster.
+cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, int cluster, cudaStream_t s);
 cudaError_t launch_paged_chunk(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
 cudaError_t launch_paged_f32(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);
 cudaError_t launch_paged_combine(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);

@@ -10,7 +10,11 @@
 //                   p = 2^(s scale log2 e - m) in f32, split into a high and a low 16-bit part
 //                   (P V then has 22 bits of p in f16, 16 in bf16, at no time that shows), O += P V
 //   item end        the 4 warps' maxima, sums and outputs are joined through shared memory.
-// The work is cut evenly over the CTAs along the positions (sc_paged.cuh).
+// Long sequences: the work is cut evenly over the CTAs along the positions (sc_paged.cuh) and the pieces are joined
+// by a second kernel.  Where no sequence has more than kClusterKeys positions, finding the cut and that kernel
+// cost more than they even out: each (sequence, KV head) then goes to a cluster of 1 to 8 CTAs, as many as keep the
+// launch within one wave, which divide its tiles and join them through distributed shared memory.
+// One sequence of 640 positions: 10.0 us cut, COMPARE1 in clusters; 64 of 513..768: 26.0 us, COMPARE2.
 #include <atomic>
 #include <type_traits>
 
@@ -61,9 +65,19 @@ struct alignas(64) DecodeParams {
     CUtensorMap kmap, vmap;
     PagedLaunch a;
     int box_shift;         // log2 of the rows of a box
+    int cluster;           // CTAs of an item (the clustered kernel)
 };
 
-template <typename T, int kHd>
+__device__ __forceinline__ float4 ld_dsmem_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+template <typename T, int kHd, bool kCluster>
 __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const __grid_constant__ DecodeParams P) {
     using C = DecCfg<kHd>;
     using M = Pack16<T>;
@@ -71,6 +85,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
     __shared__ float s_m[C::kWarps][16], s_l[C::kWarps][16];
+    __shared__ float s_ml[16][2];
     __shared__ PagedCut cut;
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* s_o = reinterpret_cast<float*>(smem + C::kStages * 2 * C::kTile);  // [warp][16][kJoinDims]
@@ -91,14 +106,38 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
     }
     pdl_launch_dependents();
     pdl_wait();
-    paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);  // synchronises the block
     PagedWalk w;
-    w.begin(cut, tt);
+    const int cs = kCluster ? P.cluster : 1, rank = kCluster ? static_cast<int>(blockIdx.x) % cs : 0;
+    if constexpr (kCluster) {
+        const int item = static_cast<int>(blockIdx.x) / cs;
+        w.b = item / kv.nkv;
+        w.h = item - w.b * kv.nkv;
+        w.rt = 0;
+        w.s = paged_seq(kv, w.b, A.max_q);
+        if (w.s.q_len == 0) return;  // the whole cluster
+        w.tiles = paged_key_tiles(w.s, 0, tt, C::kKeys);
+        w.t0 = w.tiles * rank / cs;
+        w.t1 = w.tiles * (rank + 1) / cs;
+        __syncthreads();  // the barriers are there
+    } else {
+        paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);  // synchronises the block
+        w.begin(cut, tt);
+    }
+    bool item_left = true;  // a cluster's CTA has one item
+    auto next_item = [&]() {
+        if constexpr (kCluster) {
+            const bool r = item_left;
+            item_left = false;
+            return r;
+        } else {
+            return w.next(kv, A.max_q, tt, C::kKeys);
+        }
+    };
 
     if (warp == C::kWarps) {
         // ---- producer: the whole warp, a box per lane
         int it = 0, issued = 0;
-        while (w.next(kv, A.max_q, tt, C::kKeys)) {
+        while (next_item()) {
             const int page_shift = kv.page_shift, bs = P.box_shift;
             const int last = min((w.rt + 1) * tt, w.s.q_len);
             const int keys = w.s.kv_len - w.s.q_len + last;  // positions the item's rows attend
@@ -151,6 +190,11 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
         if (lane == 0)
             for (int i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
                 mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, nullptr, kDrainNs);
+        __syncwarp();
+        if (kCluster && cs > 1) {  // with the consumers' two
+            cluster_sync();
+            cluster_sync();
+        }
         return;
     }
 
@@ -165,7 +209,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
     PagedJoin join{0, 0, 0, 0, 0};
     int it = 0;
     bool late = false;
-    while (w.next(kv, A.max_q, tt, C::kKeys)) {
+    while (next_item()) {
         // this thread's two rows
         int tok[2];
         uint32_t qa[kSteps][4];
@@ -304,8 +348,9 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
         for (int i = 0; i < C::kWarps; ++i) ll += s_m[i][row] == -INFINITY ? 0.0f : s_l[i][row] * ex2(s_m[i][row] - mm);
         const int ot = written.token(w.rt, tt, w.s.q_len);
         const int64_t orow = (w.s.row0 + (ot < 0 ? 0 : ot)) * kv.nh + w.h * G + written.g;
-        const bool whole = w.whole();
+        const bool whole = kCluster ? cs == 1 : w.whole();
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + w.slot();
+        float* s_part = reinterpret_cast<float*>(smem);  // a cluster CTA's rows, where the ring was: every tile has been read
         const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
 #pragma unroll
         for (int d0 = 0; d0 < kHd; d0 += C::kJoinDims) {
@@ -331,6 +376,8 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                 if (ot >= 0)
                     *reinterpret_cast<uint2*>(static_cast<T*>(A.o.out) + orow * kHd + d0 + cq) =
                         make_uint2(M::pack(v.x * inv, v.y * inv), M::pack(v.z * inv, v.w * inv));
+            } else if constexpr (kCluster) {
+                *reinterpret_cast<float4*>(s_part + row * kHd + d0 + cq) = v;
             } else {
                 *reinterpret_cast<float4*>(A.sc.o + (slot * 16 + row) * kHd + d0 + cq) = v;
             }
@@ -339,14 +386,62 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
         if ((tid & 7) == 0) {
             if (whole) {
                 if (A.o.lse && ot >= 0) A.o.lse[orow] = ll > 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+            } else if constexpr (kCluster) {
+                s_ml[row][0] = mm;
+                s_ml[row][1] = ll;
             } else {
                 *reinterpret_cast<float2*>(A.sc.ml + (slot * 16 + row) * 2) = make_float2(mm, ll);
             }
         }
-        if (!whole && w.t0 == 0)
+        if constexpr (kCluster) {
+            if (cs > 1) {
+                __syncwarp();
+                cluster_sync();
+                // this CTA's share of the rows' 16-byte columns: the pieces in order, weighted by 2^(m_i - m)
+                constexpr int kQuads = 16 * kHd / 4;
+                for (int i = kQuads * rank / cs + tid; i < kQuads * (rank + 1) / cs; i += 128) {
+                    const int r = i / (kHd / 4), c = i % (kHd / 4) * 4;
+                    float mi[8], li[8];
+                    float4 u[8];
+#pragma unroll
+                    for (int p = 0; p < 8; ++p) {
+                        mi[p] = -INFINITY;
+                        if (p < cs) {
+                            mi[p] = ld_dsmem_f32(dsmem_addr(&s_ml[r][0], p));
+                            li[p] = ld_dsmem_f32(dsmem_addr(&s_ml[r][1], p));
+                            u[p] = ld_dsmem_v4(dsmem_addr(s_part + r * kHd + c, p));
+                        }
+                    }
+                    float m_all = -INFINITY, l_all = 0.0f;
+#pragma unroll
+                    for (int p = 0; p < 8; ++p) m_all = fmaxf(m_all, mi[p]);
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int p = 0; p < 8; ++p)
+                        if (mi[p] > -INFINITY) {
+                            const float f = ex2(mi[p] - m_all);
+                            l_all += f * li[p];
+                            x.x += f * u[p].x;
+                            x.y += f * u[p].y;
+                            x.z += f * u[p].z;
+                            x.w += f * u[p].w;
+                        }
+                    const PagedRow pr(r, 16, G);
+                    const int t = pr.token(0, tt, w.s.q_len);
+                    if (t < 0) continue;
+                    const float f = l_all > 0.0f ? 1.0f / l_all : 0.0f;
+                    const int64_t at = (w.s.row0 + t) * kv.nh + w.h * G + pr.g;
+                    *reinterpret_cast<uint2*>(static_cast<T*>(A.o.out) + at * kHd + c) =
+                        make_uint2(M::pack(x.x * f, x.y * f), M::pack(x.z * f, x.w * f));
+                    if (A.o.lse && c == 0) A.o.lse[at] = l_all > 0.0f ? (m_all + log2f(l_all)) * 0.69314718055994531f : -INFINITY;
+                }
+                __syncwarp();
+                cluster_sync();  // no CTA leaves while another reads from it
+            }
+        } else if (!whole && w.t0 == 0)
             join = PagedJoin{w.s.row0, w.s.q_len, w.h, w.rt, w.pieces(cut)};
     }
-    if (tid == 0) A.sc.join[blockIdx.x] = join;
+    if (!kCluster && tid == 0) A.sc.join[blockIdx.x] = join;
 }
 
 // ---------------------------------------------------------------- joining the pieces of cut items
@@ -440,15 +535,36 @@ cudaError_t launch_paged_combine(const PagedLaunch& a, int out_dtype, int hd, in
 template <typename T, int kHd>
 static cudaError_t launch_decode_t(const DecodeParams& p, int ctas, cudaStream_t s) {
     using C = DecCfg<kHd>;
-    static std::atomic<uint64_t> flags{0};
-    cudaError_t e = paged_allow_smem(k_paged_decode<T, kHd>, flags, C::kSmem);
+    static std::atomic<uint64_t> flags{0}, flags_cluster{0};
+    if (p.cluster == 0) {
+        cudaError_t e = paged_allow_smem(k_paged_decode<T, kHd, false>, flags, C::kSmem);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(k_paged_decode<T, kHd, false>, dim3(static_cast<unsigned>(ctas)), dim3(C::kThreads), C::kSmem, s, p);
+    }
+    cudaError_t e = paged_allow_smem(k_paged_decode<T, kHd, true>, flags_cluster, C::kSmem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_decode<T, kHd>, dim3(static_cast<unsigned>(ctas)), dim3(C::kThreads), C::kSmem, s, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return cudaLaunchKernelEx(&cfg, k_paged_decode<T, kHd, true>, p);
 }
 
-cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s) {
+cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, int cluster, cudaStream_t s) {
     DecodeParams p;
     p.a = a;
+    p.cluster = cluster;
     p.box_shift = a.c.page_shift < 6 ? a.c.page_shift : 6;
     cudaError_t e = paged_tensor_map(&p.kmap, a.c, a.c.k, dtype, hd, 1 << p.box_shift);
     if (e == cudaSuccess) e = paged_tensor_map(&p.vmap, a.c, a.c.v, dtype, hd, 1 << p.box_shift);

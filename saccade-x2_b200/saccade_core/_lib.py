@@ -127,7 +127,7 @@ SIGNATURES_QWEN2 = {
     "sc_qwen2_f16_to_f32": (_int, [_vp, _i64, _vp, _vp]),
     "sc_qwen2_paged_append": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _int, _int, _int, _vp,
                                      _vp, _int, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
-    "sc_qwen2_paged_attention_scratch": (ctypes.c_size_t, [_i64, _i64, _int, _int, _int, _i64, _int]),
+    "sc_qwen2_paged_attention_scratch": (ctypes.c_size_t, [_i64, _int, _int, _int, _i64, _i64, _int]),
     "sc_qwen2_paged_attention": (_int, [_vp, _i64, _vp, _vp, _int, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64, _i64,
                                         _int, _int, _int, _i64, _i64, _f32, _vp, _int, _vp, _vp, ctypes.c_size_t, _vp,
                                         _vp]),

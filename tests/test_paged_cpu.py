@@ -65,7 +65,7 @@ class Call:
     def attention(self, **kw):
         p = self.p
         a = dict(q=p, qs=256, kp=p, vp=p, dtype=_lib.SC_F16, pages=4, stride=2 * 16 * 64, page=16, table=p, max_pages=4,
-                 cu=p, kv=p, seqs=1, tokens=4, nh=4, nkv=2, hd=64, max_q=1, max_kv=64, scale=0.125, out=p,
+                 cu=p, kv=p, seqs=1, tokens=4, nh=4, nkv=2, hd=64, max_q=1, max_kv=1 << 20, scale=0.125, out=p,
                  out_dtype=_lib.SC_F16, lse=None, scratch=p, nbytes=1 << 40, status=None, stream=None) | kw
         return _lib.LIB.sc_qwen2_paged_attention(*a.values())
 
@@ -117,10 +117,11 @@ def test_attention_refuses_misplaced_tensors_and_small_scratch():
     c = Call()
     for name in ("q", "kp", "vp", "out", "scratch"):
         assert c.attention(**{name: c.p + 8}) == _lib.SC_EINVAL
-    size = _lib.LIB.sc_qwen2_paged_attention_scratch(4, 1, 4, 2, 64, 1, _lib.SC_F16)
+    size = _lib.LIB.sc_qwen2_paged_attention_scratch(1, 4, 2, 64, 1, 1 << 20, _lib.SC_F16)
     assert size > 0 and c.attention(nbytes=size - 1) == _lib.SC_ENOMEM
     assert c.attention(tokens=0) == _lib.SC_OK
-    assert _lib.LIB.sc_qwen2_paged_attention_scratch(4, 1, 3, 2, 64, 1, _lib.SC_F16) == 0
+    assert _lib.LIB.sc_qwen2_paged_attention_scratch(1, 3, 2, 64, 1, 1 << 20, _lib.SC_F16) == 0  # refused
+    assert _lib.LIB.sc_qwen2_paged_attention_scratch(1, 4, 2, 64, 1, 100, _lib.SC_F16) == 0  # none wanted
 
 
 @pytest.mark.parametrize("kw", [

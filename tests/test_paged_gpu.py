@@ -21,6 +21,7 @@ def sc():
 
 
 def attend(sc, c, **kw):
+    """The call, with length bounds of its own if the case has them."""
     out = torch.full((c.tokens, c.nh, c.hd), 7.0, dtype=kw.pop("out_dtype", c.dtype), device=c.q.device)
     status = torch.zeros(1, dtype=torch.int32, device=c.q.device)
     got, lse = sc.paged_attention(c.q, c.k_pages, c.v_pages, c.table, c.cu_q, c.kv_len, c.max_q, c.max_kv, out=out,
@@ -58,11 +59,21 @@ LENS = {
 @pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (3, 1, 128), (8, 8, 64), (16, 2, 128), (20, 1, 64)],
                          ids=lambda h: "x".join(map(str, h)))
 @pytest.mark.parametrize("lens", list(LENS), ids=list(LENS))
-def test_attention_matches_64_bits(sc, dtype, heads, lens):
+def test_attention_matches_64_bits(sc, dtype, heads, lens, bound=None):
     page = {"decode": 16, "decode-long": 64, "ragged": 8, "chunk": 32, "short": 128, "one": 256, "none": 8}[lens]
     c = Paged(LENS[lens], *heads, page, dtype, "cuda", seed=len(lens) + heads[0], behind=3)
+    c.max_kv = bound or c.max_kv
     scale = heads[2] ** -0.5
     compare(c, *attend(sc, c), scale)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (20, 1, 64)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("lens", ["decode", "short", "one", "none", "decode-long"])
+@pytest.mark.parametrize("bound", [1, 200, 2048, 1 << 24])
+def test_any_bound_on_the_positions_gives_the_attention(sc, dtype, heads, lens, bound):
+    """The bound chooses between clusters (of 1 to 8 CTAs) and the cut line; sequences may even exceed it."""
+    test_attention_matches_64_bits(sc, dtype, heads, lens, bound)
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
