@@ -286,11 +286,12 @@ static PagedPlan paged_plan(int dtype, int64_t num_seqs, int nh, int nkv, int hd
         p.kind = PagedPlan::kDecode;
         p.ctas = 2 * sms;
         p.tl = {16, 16, 16 / G, 64};
-        if (max_kv <= kClusterKeys) {
-            const int64_t items = num_seqs * nkv;
-            p.cluster = 1;
-            while (p.cluster < 8 && items * p.cluster * 2 <= p.ctas && p.cluster * 2 * p.tl.kt <= max_kv) p.cluster *= 2;
-            p.ctas = items * p.cluster;
+        const int64_t items = num_seqs * nkv;
+        int cs = 1;
+        while (cs < 8 && items * cs * 2 <= p.ctas && cs * 2 * p.tl.kt <= max_kv) cs *= 2;
+        if (max_kv <= kClusterKeys * cs) {
+            p.cluster = cs;
+            p.ctas = items * cs;
         }
     } else {
         p.kind = PagedPlan::kChunk;

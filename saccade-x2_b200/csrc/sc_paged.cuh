@@ -13,7 +13,7 @@
 
 namespace sc {
 
-constexpr int64_t kClusterKeys = 2048;  // positions up to which few new tokens go to clusters
+constexpr int64_t kClusterKeys = 2048;  // positions of a clustered CTA's share at most (sc_paged_decode.cu)
 constexpr int kPagedMaxGroup = 64;     // query heads per KV head
 constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
 
