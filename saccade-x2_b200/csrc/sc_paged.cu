@@ -278,25 +278,30 @@ static PagedPlan paged_plan(int dtype, int64_t num_seqs, int nh, int nkv, int hd
     const int G = nh / nkv, sms = sm_count();
     const bool few = max_q * G <= 16;
     PagedPlan p{};
+    int64_t share = 0;  // positions of a clustered CTA at most
     if (dtype == SC_F32) {
         p.kind = PagedPlan::kF32;
         p.ctas = few || hd == 64 ? 2 * sms : sms;
         p.tl = few ? PagedTiling{16, 16, 16 / G, 64} : PagedTiling{64, 64, 64 / G, 64};
+        share = few ? kClusterKeysF32 : 0;
     } else if (few) {
         p.kind = PagedPlan::kDecode;
         p.ctas = 2 * sms;
         p.tl = {16, 16, 16 / G, 64};
-        const int64_t items = num_seqs * nkv;
-        int cs = 1;
-        while (cs < 8 && items * cs * 2 <= p.ctas && cs * 2 * p.tl.kt <= max_kv) cs *= 2;
-        if (max_kv <= kClusterKeys * cs) {
-            p.cluster = cs;
-            p.ctas = items * cs;
-        }
+        share = kClusterKeys;
     } else {
         p.kind = PagedPlan::kChunk;
         p.ctas = sms;
         p.tl = {256, 128, 2 * (128 / G), 128};
+    }
+    if (share > 0) {
+        const int64_t items = num_seqs * nkv * ((max_q + p.tl.tt - 1) / p.tl.tt);
+        int cs = 1;
+        while (cs < 8 && items * cs * 2 <= p.ctas && cs * 2 * p.tl.kt <= max_kv) cs *= 2;
+        if (max_kv <= share * cs && items <= 1 << 20) {
+            p.cluster = cs;
+            p.ctas = items * cs;
+        }
     }
     if (p.cluster == 0) p.scratch = paged_scratch_bytes(p.ctas, p.tl.rows, hd);
     return p;
@@ -448,7 +453,7 @@ sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* 
     const int ctas = static_cast<int>(p.ctas);
     const PagedLaunch a{c, q, q_stride, max_q_len, {out, lse, scale * 1.4426950408889634f}, p.tl,
                         paged_scratch(scratch, p.cluster ? 0 : p.ctas, p.tl.rows, head_dim)};
-    cudaError_t e = p.kind == PagedPlan::kF32      ? launch_paged_f32(a, out_dtype, head_dim, ctas, s)
+    cudaError_t e = p.kind == PagedPlan::kF32      ? launch_paged_f32(a, out_dtype, head_dim, ctas, p.cluster, s)
                     : p.kind == PagedPlan::kDecode ? launch_paged_decode(a, cache_dtype, head_dim, ctas, p.cluster, s)
                                                    : launch_paged_chunk(a, cache_dtype, head_dim, ctas, s);
     if (e == cudaSuccess && p.cluster == 0) e = launch_paged_combine(a, out_dtype, head_dim, ctas, s);

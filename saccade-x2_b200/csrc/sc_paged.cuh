@@ -7,13 +7,15 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "sc_device.cuh"
 #include "sc_internal.h"
 
 namespace sc {
 
-constexpr int64_t kClusterKeys = 2048;  // positions of a clustered CTA's share at most (sc_paged_decode.cu)
+constexpr int64_t kClusterKeys = 2048;     // positions of a clustered CTA's share at most (sc_paged_decode.cu)
+constexpr int64_t kClusterKeysF32 = 128;  // (sc_paged_f32.cu)
 constexpr int kPagedMaxGroup = 64;     // query heads per KV head
 constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
 
@@ -314,6 +316,15 @@ __device__ __forceinline__ void tma_page(void* smem_dst, const CUtensorMap* map,
         : "memory");
 }
 
+__device__ __forceinline__ float4 ld_dsmem_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
 struct PagedLaunch {
     PagedKv c;
     const void* q;
@@ -343,10 +354,32 @@ cudaError_t paged_allow_smem(Kern kern, std::atomic<uint64_t>& flags, int bytes)
     return e;
 }
 
+// A launch of `ctas` CTAs in clusters, with programmatic stream serialization.
+template <typename Params>
+cudaError_t paged_launch_clusters(void (*kernel)(Params), int ctas, int threads, int smem, int cluster, cudaStream_t s,
+                                  const std::remove_const_t<Params>& p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 // cluster 0: the line cut into `ctas` pieces; otherwise ctas = items * cluster.
 cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, int cluster, cudaStream_t s);
 cudaError_t launch_paged_chunk(const PagedLaunch& a, int dtype, int hd, int ctas, cudaStream_t s);
-cudaError_t launch_paged_f32(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);
+cudaError_t launch_paged_f32(const PagedLaunch& a, int out_dtype, int hd, int ctas, int cluster, cudaStream_t s);
 cudaError_t launch_paged_combine(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s);
 
 }  // namespace sc

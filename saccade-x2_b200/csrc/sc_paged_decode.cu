@@ -70,15 +70,6 @@ struct alignas(64) DecodeParams {
     int cluster;           // CTAs of an item (the clustered kernel)
 };
 
-__device__ __forceinline__ float4 ld_dsmem_v4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-
 template <typename T, int kHd, bool kCluster>
 __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const __grid_constant__ DecodeParams P) {
     using C = DecCfg<kHd>;
@@ -545,22 +536,7 @@ static cudaError_t launch_decode_t(const DecodeParams& p, int ctas, cudaStream_t
     }
     cudaError_t e = paged_allow_smem(k_paged_decode<T, kHd, true>, flags_cluster, C::kSmem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = C::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return cudaLaunchKernelEx(&cfg, k_paged_decode<T, kHd, true>, p);
+    return paged_launch_clusters(k_paged_decode<T, kHd, true>, ctas, C::kThreads, C::kSmem, p.cluster, s, p);
 }
 
 cudaError_t launch_paged_decode(const PagedLaunch& a, int dtype, int hd, int ctas, int cluster, cudaStream_t s) {

@@ -7,7 +7,11 @@
 // with a running maximum and sum of its own, joined at the item's end, so that every thread keeps 4 rows.
 // K and V tiles of 64 positions come by 16-byte asynchronous copies, the next K while O is updated, the
 // next V while S is computed; rows padded by 16 bytes keep 8 of them on different banks.  Positions behind
-// the last one are zero-filled.  Pieces of the line of key tiles go to the CTAs evenly (sc_paged.cuh).
+// the last one are zero-filled.  Pieces of the line of key tiles go to the CTAs evenly (sc_paged.cuh); few new
+// tokens whose CTAs would have at most kClusterKeysF32 positions each go to clusters as in sc_paged_decode.cu (one
+// sequence of 1..256 positions, 28 + 4 heads of 128: 12.2 us cut, 8.4 us in clusters; 4 of 513..1024 16.2 and 18.5;
+// row tiles of 64 rows, bound by their arithmetic, want the even cut: 12 sequences of 1..24 new tokens over up to
+// 1500 positions 34 us cut, 56 us in clusters of 4).
 #include <atomic>
 #include <type_traits>
 
@@ -50,27 +54,59 @@ struct F32Cfg {
     static constexpr int kSmem = (kQ + 2 * kKv + kP) * 4;
 };
 
-template <typename Out, int kRows, int kHd>
-__global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged_f32(const PagedLaunch A) {
+// kCluster: an item (sequence, KV head, row tile) per cluster of P.cluster CTAs, which divide its key tiles and join
+// them through distributed shared memory; otherwise a piece of the line per CTA.
+struct F32Params {
+    PagedLaunch a;
+    int cluster;
+    int rts;      // row tiles of a sequence at most (clusters beyond a sequence's own leave)
+};
+
+template <typename Out, int kRows, int kHd, bool kCluster>
+__global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged_f32(const F32Params P) {
     using C = F32Cfg<kRows, kHd>;
+    const PagedLaunch& A = P.a;
     constexpr int kC8 = kHd / 16;  // columns of O of a thread: 4 at 4 tx + 64 i
     extern __shared__ __align__(16) float sm[];
     __shared__ PagedCut cut;
-    __shared__ float s_m[C::kGroups][kRows], s_l[C::kGroups][kRows];
+    __shared__ float s_m[C::kGroups][kRows], s_l[C::kGroups][kRows], s_ml[kRows][2];
     float *sq = sm, *sk = sm + C::kQ, *sv = sk + C::kKv, *sp = sv + C::kKv;
     const PagedKv& kv = A.c;
     const int tid = threadIdx.x, G = kv.nh / kv.nkv, tt = A.tl.tt;
     const int tx = tid & 15, ty = (tid >> 4) % (kRows / 4), grp = tid / (kRows * 4);
     pdl_launch_dependents();
     pdl_wait();
-    paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);
     PagedWalk w;
-    w.begin(cut, tt);
+    const int cs = kCluster ? P.cluster : 1, rank = kCluster ? static_cast<int>(blockIdx.x) % cs : 0;
+    if constexpr (kCluster) {
+        const int item = static_cast<int>(blockIdx.x) / cs, head = item / P.rts;
+        w.rt = item - head * P.rts;
+        w.b = head / kv.nkv;
+        w.h = head - w.b * kv.nkv;
+        w.s = paged_seq(kv, w.b, A.max_q);
+        if (w.rt >= paged_row_tiles(w.s, tt)) return;  // the whole cluster
+        w.tiles = paged_key_tiles(w.s, w.rt, tt, C::kKeys);
+        w.t0 = w.tiles * rank / cs;
+        w.t1 = w.tiles * (rank + 1) / cs;
+    } else {
+        paged_cut<C::kThreads>(kv, A.max_q, tt, C::kKeys, &cut);
+        w.begin(cut, tt);
+    }
+    bool item_left = true;  // a cluster's CTA has one item
+    auto next_item = [&]() {
+        if constexpr (kCluster) {
+            const bool r = item_left;
+            item_left = false;
+            return r;
+        } else {
+            return w.next(kv, A.max_q, tt, C::kKeys);
+        }
+    };
     const PagedRow mine[4] = {PagedRow(ty * 4, kRows, G), PagedRow(ty * 4 + 1, kRows, G), PagedRow(ty * 4 + 2, kRows, G),
                               PagedRow(ty * 4 + 3, kRows, G)};
     PagedJoin join{0, 0, 0, 0, 0};
     const float sl2 = A.o.sl2;
-    while (w.next(kv, A.max_q, tt, C::kKeys)) {
+    while (next_item()) {
         const int start = w.s.kv_len - w.s.q_len;
         const int keys = start + min((w.rt + 1) * tt, w.s.q_len);
         const int32_t* table = kv.table + w.b * kv.max_pages;
@@ -107,7 +143,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                 cp16(d0 + j * kStep * C::kLd * 4, static_cast<const float*>(pages) + (place[j] < 0 ? 0 : place[j]), place[j] >= 0);
             cp_commit();
         };
-        look_up(w.t0);
+        if (w.t0 < w.t1) look_up(w.t0);  // (a cluster's CTA may have none)
         constexpr int kQueries = kRows * (kHd / 4) / C::kThreads;
         float4 qv[kQueries];
 #pragma unroll
@@ -119,10 +155,12 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                 qv[j] = *reinterpret_cast<const float4*>(static_cast<const float*>(A.q) + (w.s.row0 + tok) * A.q_stride +
                                                          (w.h * G + row.g) * kHd + cc);
         }
-        find(w.t0);
         __syncthreads();  // the item before has read its tiles
-        load(kv.k, sk);
-        load(kv.v, sv);
+        if (w.t0 < w.t1) {
+            find(w.t0);
+            load(kv.k, sk);
+            load(kv.v, sv);
+        }
 #pragma unroll
         for (int j = 0; j < kQueries; ++j) *reinterpret_cast<float4*>(sq + (cr + kStep * j) * C::kLd + cc) = qv[j];
         int pos[4];
@@ -238,9 +276,15 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                 s_l[grp][ty * 4 + i] = l[i];
             }
         }
-        const bool whole = w.whole();
+        if (kCluster) __syncthreads();  // (K's and V's place is written again)
+        const bool whole = kCluster ? cs == 1 : w.whole();
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + w.slot();
         auto write = [&](int row, int col, float4 v, float mm, float ll) {  // 4 columns of a row, and its sums once
+            if (kCluster && !whole) {  // where K was: every tile has been read
+                *reinterpret_cast<float4*>(sk + row * kHd + col) = v;
+                if (col == 0) s_ml[row][0] = mm, s_ml[row][1] = ll;
+                return;
+            }
             const PagedRow r(row, kRows, G);
             const int tok = r.token(w.rt, tt, w.s.q_len);
             if (tok < 0) return;
@@ -298,30 +342,85 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                 write(row, col, v, mm, ll);
             }
         }
-        if (!whole && w.t0 == 0)
+        if constexpr (kCluster) {
+            if (cs > 1) {
+                __syncwarp();
+                cluster_sync();
+                // this CTA's share of the rows' 16-byte columns: the pieces in order, weighted by 2^(m_i - m)
+                constexpr int kQuads = kRows * kHd / 4;
+                for (int i = kQuads * rank / cs + tid; i < kQuads * (rank + 1) / cs; i += C::kThreads) {
+                    const int row = i / (kHd / 4), col = i % (kHd / 4) * 4;
+                    float mi[8], li[8];
+                    float4 u[8];
+#pragma unroll
+                    for (int p = 0; p < 8; ++p) {
+                        mi[p] = -INFINITY;
+                        if (p < cs) {
+                            mi[p] = ld_dsmem_f32(dsmem_addr(&s_ml[row][0], p));
+                            li[p] = ld_dsmem_f32(dsmem_addr(&s_ml[row][1], p));
+                            u[p] = ld_dsmem_v4(dsmem_addr(sk + row * kHd + col, p));
+                        }
+                    }
+                    float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+                    for (int p = 0; p < 8; ++p) mm = fmaxf(mm, mi[p]);
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int p = 0; p < 8; ++p)
+                        if (mi[p] > -INFINITY) {
+                            const float f = ex2(mi[p] - mm);
+                            ll += f * li[p];
+                            x.x += f * u[p].x;
+                            x.y += f * u[p].y;
+                            x.z += f * u[p].z;
+                            x.w += f * u[p].w;
+                        }
+                    const PagedRow r(row, kRows, G);
+                    const int tok = r.token(w.rt, tt, w.s.q_len);
+                    if (tok < 0) continue;
+                    const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+                    const int64_t orow = (w.s.row0 + tok) * kv.nh + w.h * G + r.g;
+                    x.x *= inv, x.y *= inv, x.z *= inv, x.w *= inv;
+                    if constexpr (std::is_same<Out, __half>::value)
+                        *reinterpret_cast<uint2*>(static_cast<__half*>(A.o.out) + orow * kHd + col) =
+                            make_uint2(Pack16<__half>::pack(x.x, x.y), Pack16<__half>::pack(x.z, x.w));
+                    else
+                        *reinterpret_cast<float4*>(static_cast<float*>(A.o.out) + orow * kHd + col) = x;
+                    if (col == 0 && A.o.lse) A.o.lse[orow] = ll > 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+                }
+                __syncwarp();
+                cluster_sync();  // no CTA leaves while another reads from it
+            }
+        } else if (!whole && w.t0 == 0)
             join = PagedJoin{w.s.row0, w.s.q_len, w.h, w.rt, w.pieces(cut)};
     }
-    if (tid == 0) A.sc.join[blockIdx.x] = join;
+    if (!kCluster && tid == 0) A.sc.join[blockIdx.x] = join;
 }
 
 template <typename Out, int kRows, int kHd>
-static cudaError_t launch_f32_t(const PagedLaunch& a, int ctas, cudaStream_t s) {
+static cudaError_t launch_f32_t(const F32Params& p, int ctas, cudaStream_t s) {
     using C = F32Cfg<kRows, kHd>;
-    static std::atomic<uint64_t> flags{0};
-    cudaError_t e = paged_allow_smem(k_paged_f32<Out, kRows, kHd>, flags, C::kSmem);
+    static std::atomic<uint64_t> flags{0}, flags_cluster{0};
+    if (p.cluster == 0) {
+        cudaError_t e = paged_allow_smem(k_paged_f32<Out, kRows, kHd, false>, flags, C::kSmem);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(k_paged_f32<Out, kRows, kHd, false>, dim3(static_cast<unsigned>(ctas)), dim3(C::kThreads), C::kSmem, s, p);
+    }
+    cudaError_t e = paged_allow_smem(k_paged_f32<Out, kRows, kHd, true>, flags_cluster, C::kSmem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_f32<Out, kRows, kHd>, dim3(static_cast<unsigned>(ctas)), dim3(C::kThreads), C::kSmem, s, a);
+    return paged_launch_clusters(k_paged_f32<Out, kRows, kHd, true>, ctas, C::kThreads, C::kSmem, p.cluster, s, p);
 }
 
-cudaError_t launch_paged_f32(const PagedLaunch& a, int out_dtype, int hd, int ctas, cudaStream_t s) {
+cudaError_t launch_paged_f32(const PagedLaunch& a, int out_dtype, int hd, int ctas, int cluster, cudaStream_t s) {
+    const F32Params p{a, cluster, static_cast<int>((a.max_q + a.tl.tt - 1) / a.tl.tt)};
     if (a.tl.rows == 16) {
         if (out_dtype == SC_F16)
-            return hd == 128 ? launch_f32_t<__half, 16, 128>(a, ctas, s) : launch_f32_t<__half, 16, 64>(a, ctas, s);
-        return hd == 128 ? launch_f32_t<float, 16, 128>(a, ctas, s) : launch_f32_t<float, 16, 64>(a, ctas, s);
+            return hd == 128 ? launch_f32_t<__half, 16, 128>(p, ctas, s) : launch_f32_t<__half, 16, 64>(p, ctas, s);
+        return hd == 128 ? launch_f32_t<float, 16, 128>(p, ctas, s) : launch_f32_t<float, 16, 64>(p, ctas, s);
     }
     if (out_dtype == SC_F16)
-        return hd == 128 ? launch_f32_t<__half, 64, 128>(a, ctas, s) : launch_f32_t<__half, 64, 64>(a, ctas, s);
-    return hd == 128 ? launch_f32_t<float, 64, 128>(a, ctas, s) : launch_f32_t<float, 64, 64>(a, ctas, s);
+        return hd == 128 ? launch_f32_t<__half, 64, 128>(p, ctas, s) : launch_f32_t<__half, 64, 64>(p, ctas, s);
+    return hd == 128 ? launch_f32_t<float, 64, 128>(p, ctas, s) : launch_f32_t<float, 64, 64>(p, ctas, s);
 }
 
 }  // namespace sc

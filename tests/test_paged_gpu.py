@@ -67,9 +67,9 @@ def test_attention_matches_64_bits(sc, dtype, heads, lens, bound=None):
     compare(c, *attend(sc, c), scale)
 
 
-@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
 @pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (20, 1, 64)], ids=lambda h: "x".join(map(str, h)))
-@pytest.mark.parametrize("lens", ["decode", "short", "one", "none", "decode-long"])
+@pytest.mark.parametrize("lens", ["decode", "short", "one", "none", "decode-long", "ragged", "chunk"])
 @pytest.mark.parametrize("bound", [1, 200, 2048, 1 << 24])
 def test_any_bound_on_the_positions_gives_the_attention(sc, dtype, heads, lens, bound):
     """The bound chooses between clusters (of 1 to 8 CTAs) and the cut line; sequences may even exceed it."""
