@@ -294,11 +294,11 @@ static PagedPlan paged_plan(int dtype, int64_t num_seqs, int nh, int nkv, int hd
         p.ctas = sms;
         p.tl = {256, 128, 2 * (128 / G), 128};
     }
-    if (share > 0) {
-        const int64_t items = num_seqs * nkv * ((max_q + p.tl.tt - 1) / p.tl.tt);
+    if (share > 0) {  // few new tokens: a row tile per sequence and KV head
+        const int64_t items = num_seqs * nkv;
         int cs = 1;
         while (cs < 8 && items * cs * 2 <= p.ctas && cs * 2 * p.tl.kt <= max_kv) cs *= 2;
-        if (max_kv <= share * cs && items <= 1 << 20) {
+        if (max_kv <= share * cs) {
             p.cluster = cs;
             p.ctas = items * cs;
         }

@@ -54,12 +54,11 @@ struct F32Cfg {
     static constexpr int kSmem = (kQ + 2 * kKv + kP) * 4;
 };
 
-// kCluster: an item (sequence, KV head, row tile) per cluster of P.cluster CTAs, which divide its key tiles and join
-// them through distributed shared memory; otherwise a piece of the line per CTA.
+// kCluster (few new tokens: one row tile): a (sequence, KV head) per cluster of P.cluster CTAs, which divide its key
+// tiles and join them through distributed shared memory; otherwise a piece of the line per CTA.
 struct F32Params {
     PagedLaunch a;
     int cluster;
-    int rts;      // row tiles of a sequence at most (clusters beyond a sequence's own leave)
 };
 
 template <typename Out, int kRows, int kHd, bool kCluster>
@@ -79,13 +78,13 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
     PagedWalk w;
     const int cs = kCluster ? P.cluster : 1, rank = kCluster ? static_cast<int>(blockIdx.x) % cs : 0;
     if constexpr (kCluster) {
-        const int item = static_cast<int>(blockIdx.x) / cs, head = item / P.rts;
-        w.rt = item - head * P.rts;
-        w.b = head / kv.nkv;
-        w.h = head - w.b * kv.nkv;
+        const int item = static_cast<int>(blockIdx.x) / cs;
+        w.b = item / kv.nkv;
+        w.h = item - w.b * kv.nkv;
+        w.rt = 0;
         w.s = paged_seq(kv, w.b, A.max_q);
-        if (w.rt >= paged_row_tiles(w.s, tt)) return;  // the whole cluster
-        w.tiles = paged_key_tiles(w.s, w.rt, tt, C::kKeys);
+        if (w.s.q_len == 0) return;  // the whole cluster
+        w.tiles = paged_key_tiles(w.s, 0, tt, C::kKeys);
         w.t0 = w.tiles * rank / cs;
         w.t1 = w.tiles * (rank + 1) / cs;
     } else {
@@ -401,18 +400,20 @@ template <typename Out, int kRows, int kHd>
 static cudaError_t launch_f32_t(const F32Params& p, int ctas, cudaStream_t s) {
     using C = F32Cfg<kRows, kHd>;
     static std::atomic<uint64_t> flags{0}, flags_cluster{0};
-    if (p.cluster == 0) {
-        cudaError_t e = paged_allow_smem(k_paged_f32<Out, kRows, kHd, false>, flags, C::kSmem);
-        if (e != cudaSuccess) return e;
-        return launch_pdl(k_paged_f32<Out, kRows, kHd, false>, dim3(static_cast<unsigned>(ctas)), dim3(C::kThreads), C::kSmem, s, p);
+    if constexpr (kRows == 16) {
+        if (p.cluster > 0) {
+            const cudaError_t e = paged_allow_smem(k_paged_f32<Out, kRows, kHd, true>, flags_cluster, C::kSmem);
+            if (e != cudaSuccess) return e;
+            return paged_launch_clusters(k_paged_f32<Out, kRows, kHd, true>, ctas, C::kThreads, C::kSmem, p.cluster, s, p);
+        }
     }
-    cudaError_t e = paged_allow_smem(k_paged_f32<Out, kRows, kHd, true>, flags_cluster, C::kSmem);
+    const cudaError_t e = paged_allow_smem(k_paged_f32<Out, kRows, kHd, false>, flags, C::kSmem);
     if (e != cudaSuccess) return e;
-    return paged_launch_clusters(k_paged_f32<Out, kRows, kHd, true>, ctas, C::kThreads, C::kSmem, p.cluster, s, p);
+    return launch_pdl(k_paged_f32<Out, kRows, kHd, false>, dim3(static_cast<unsigned>(ctas)), dim3(C::kThreads), C::kSmem, s, p);
 }
 
 cudaError_t launch_paged_f32(const PagedLaunch& a, int out_dtype, int hd, int ctas, int cluster, cudaStream_t s) {
-    const F32Params p{a, cluster, static_cast<int>((a.max_q + a.tl.tt - 1) / a.tl.tt)};
+    const F32Params p{a, cluster};
     if (a.tl.rows == 16) {
         if (out_dtype == SC_F16)
             return hd == 128 ? launch_f32_t<__half, 16, 128>(p, ctas, s) : launch_f32_t<__half, 16, 64>(p, ctas, s);
