@@ -682,6 +682,7 @@ class PagedDecoder:
         lens = [int(p.numel()) for p in prompts]
         if max(lens) > c.max_positions:
             raise ValueError(f"a prompt of {max(lens)} tokens: the cache is made for up to {c.max_positions}")
+        self.stream.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.device(dev), torch.cuda.stream(self.stream):
             for b, n in enumerate(lens):
                 c.reserve(b, n)
@@ -721,6 +722,8 @@ class PagedDecoder:
         self._take(self.last, self._choose(logits))
 
     def _reserve_next(self) -> None:
+        if min(self.lengths) < 1:
+            raise RuntimeError("start() takes the prompts first")
         if max(self.lengths) >= self.cache.max_positions:
             raise RuntimeError(f"a sequence has all of the cache's {self.cache.max_positions} positions")
         for b in range(self.B):
@@ -757,7 +760,6 @@ class PagedDecoder:
 
     def generate(self, prompts, steps: int, *, chunk: int = 2048, graph: bool = True) -> torch.Tensor:
         """Tokens [batch, steps] after the prompts."""
-        self.stream.wait_stream(torch.cuda.current_stream(self.model.device))
         out = [self.start(prompts, chunk)]
         if graph and self.graph is None and steps > 1:
             self.capture()

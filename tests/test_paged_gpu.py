@@ -89,6 +89,37 @@ def test_attention_page_sizes_strides_and_bounds(sc, dtype, page):
     compare(c, *attend(sc, c, scale=0.3), 0.3)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("bound", [64, 1 << 20])
+@pytest.mark.parametrize("q_len", [1, 3])
+def test_more_sequences_than_threads(sc, dtype, bound, q_len):
+    """A thousand short sequences, some without new tokens: the work is divided over several blocks of them.
+    (One token is few for every kernel, three tokens of 7 heads are many.)"""
+    lens = [((i % 5 != 3) * q_len, q_len + i * 7 % 41) for i in range(1000)]
+    c = Paged(lens, 14, 2, 64, 8, dtype, "cuda", seed=7, behind=2)
+    c.max_kv = bound
+    compare(c, *attend(sc, c), 0.125)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("lens", [[(1, 70), (5, 5)], [(33, 200), (1, 1)]], ids=["few", "many"])
+def test_64_query_heads_of_a_kv_head(sc, dtype, lens):
+    c = Paged(lens, 64, 1, 64, 16, dtype, "cuda", seed=21)
+    compare(c, *attend(sc, c), 0.125)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("lens", ["decode", "chunk", "ragged"])
+@pytest.mark.parametrize("bound", [None, 1 << 20])
+def test_output_over_the_queries(sc, dtype, lens, bound):
+    c = Paged(LENS[lens], 14, 2, 64, 16, dtype, "cuda", seed=31)
+    c.max_kv = bound or c.max_kv
+    want, _ = attend(sc, c)
+    q = c.q.clone()
+    assert sc.paged_attention(q, c.k_pages, c.v_pages, c.table, c.cu_q, c.kv_len, c.max_q, c.max_kv, out=q) is q
+    assert torch.equal(q, want)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
 def test_attention_extreme_scores(sc, dtype):
     """Scores of hundreds: weights from 1 down to zero, maxima that move by more than any exponent."""
@@ -128,14 +159,17 @@ def test_two_calls_are_the_same_bits_and_streams_do_not_mix(sc, lens):
     assert torch.equal(a, a0) and torch.equal(b, b0)
 
 
-def test_attention_in_a_graph_follows_lengths_and_tables(sc):
-    """A captured call replays with other lengths and pages in the same tensors."""
-    c = Paged([(1, 40), (1, 500), (1, 3)], 14, 2, 64, 16, F16, "cuda", seed=11)
-    d = Paged([(1, 333), (1, 1), (1, 511)], 14, 2, 64, 16, F16, "cuda", seed=12)
+@pytest.mark.parametrize("q_len,bound", [(1, 512), (1, 1 << 20), (60, 512)])
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+def test_attention_in_a_graph_follows_lengths_and_tables(sc, dtype, q_len, bound):
+    """A captured call replays with other lengths and pages in the same tensors, and a second graph
+    beside it on another stream does not touch its scratch."""
+    c = Paged([(q_len, 140), (q_len, 500), (q_len, 63)], 14, 2, 64, 16, dtype, "cuda", seed=11)
+    d = Paged([(q_len, 333), (q_len, 60), (q_len, 511)], 14, 2, 64, 16, dtype, "cuda", seed=12)
     width = max(c.table.shape[1], d.table.shape[1])
     table = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
     pages = max(c.pages, d.pages)
-    kp = torch.full((pages, 2, 16, 64), math.nan, dtype=F16, device="cuda")
+    kp = torch.full((pages, 2, 16, 64), math.nan, dtype=dtype, device="cuda")
     vp, q, kv, cu = kp.clone(), torch.empty_like(c.q), c.kv_len.clone(), c.cu_q.clone()
 
     def fill(x):
@@ -146,18 +180,24 @@ def test_attention_in_a_graph_follows_lengths_and_tables(sc):
     fill(c)
     stream = torch.cuda.Stream()
     with torch.cuda.stream(stream):
-        sc.paged_attention(q, kp, vp, table, cu, kv, 1, 512)
+        sc.paged_attention(q, kp, vp, table, cu, kv, q_len, bound)
     stream.synchronize()
-    graph = torch.cuda.CUDAGraph()
+    graph, other, side = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
     with torch.cuda.graph(graph, stream=stream):
-        got = sc.paged_attention(q, kp, vp, table, cu, kv, 1, 512)
+        got = sc.paged_attention(q, kp, vp, table, cu, kv, q_len, bound)
+    with torch.cuda.graph(other, stream=side):
+        beside = sc.paged_attention(d.q, d.k_pages, d.v_pages, d.table, d.cu_q, d.kv_len, q_len, bound)
+    want = {x: sc.paged_attention(x.q, x.k_pages, x.v_pages, x.table, x.cu_q, x.kv_len, q_len, bound) for x in (c, d)}
     for x in (c, d, c):
         fill(x)
         torch.cuda.synchronize()
-        graph.replay()
+        for _ in range(3):
+            with torch.cuda.stream(side):
+                other.replay()
+            with torch.cuda.stream(stream):
+                graph.replay()
         torch.cuda.synchronize()
-        want = sc.paged_attention(x.q, x.k_pages, x.v_pages, x.table, x.cu_q, x.kv_len, 1, 512)
-        assert torch.equal(got, want)
+        assert torch.equal(got, want[x]) and torch.equal(beside, want[d])
 
 
 @pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
@@ -256,6 +296,19 @@ def test_append_matches_64_bits(sc, src, dtype, heads, layout):
     if src == dtype and layout == "apart":  # in place: the same bits
         sc.paged_append(q, k, v, cos, sin, kp, vp, c.table, c.cu_q, c.kv_len, out=q)
         assert torch.equal(q[:c.cu[-1]], out[:c.cu[-1]])
+
+
+def test_append_for_more_sequences_than_a_warp(sc):
+    lens = [(i % 3, 1 + i % 3 + i % 29) for i in range(300)]
+    c = Paged(lens, 4, 2, 64, 8, F16, "cuda", seed=1)
+    q, k, v = (torch.randn(c.tokens, n, 64, device="cuda") for n in (4, 2, 2))
+    cos, sin = tables(40, 64, "cuda")
+    kp, vp = torch.zeros_like(c.k_pages), torch.zeros_like(c.v_pages)
+    sc.paged_append(q, k, v, cos, sin, kp, vp, c.table, c.cu_q, c.kv_len)
+    for b, (n, kv) in enumerate(lens):
+        for i in range(n):
+            p, row = kv - n + i, c.cu[b] + i
+            assert torch.equal(vp[int(c.table[b, p // 8]), :, p % 8], v[row].half())
 
 
 def test_append_skips_what_has_no_place(sc):

@@ -163,6 +163,10 @@ def test_decoder_refusals(q2, ck):
     with pytest.raises(ValueError):
         q2.Qwen2Model(ck, max_pos=32, cache=cache)
     dec = q2.PagedDecoder(model, 1)
+    with pytest.raises(RuntimeError):
+        dec.step()  # before any prompt
+    with pytest.raises(RuntimeError):
+        dec.capture()
     dec.start(prompts([47], 100, 1))
     dec.step()
     with pytest.raises(RuntimeError):
