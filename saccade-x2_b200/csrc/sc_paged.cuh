@@ -222,6 +222,49 @@ struct PagedWalk {
     }
 };
 
+// ---------------------------------------------------------------- values that are not finite
+// A row must not see the values of positions behind its own, but the products give them the weight 0, and
+// 0 * inf is NaN.  The positions that some rows of an item attend and others do not are the item's own new
+// tokens.  The kernels look their values over where they are staged, replace what is not finite by 0, and, once
+// a CTA has met such a value, add these tokens' to the rows that do attend them after the rows have been
+// written (inf or NaN, as the formula has them).
+
+// Adds the values that are not finite of positions first .. last to columns c0 + kStep i .. + 3 of a written row.
+template <typename T, int kHd, int kStep, typename Out>
+__device__ __forceinline__ void paged_add_not_finite(const PagedKv& p, int b, int h, int first, int last, int c0, Out* row) {
+#pragma unroll 1
+    for (int key = first; key <= last; ++key) {
+        const int64_t page = p.table[b * p.max_pages + (key >> p.page_shift)];
+        if (page < 0 || page >= p.num_pages) continue;
+        const T* v = static_cast<const T*>(p.v) + page * p.page_stride +
+                     ((static_cast<int64_t>(h) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * kHd;
+#pragma unroll 1
+        for (int i = c0; i < kHd; i += kStep)
+#pragma unroll 1
+            for (int c = i; c < i + 4; ++c) {
+                const float x = static_cast<float>(v[c]);
+                if (!(x - x == 0.0f)) row[c] = static_cast<Out>(static_cast<float>(row[c]) + x);
+            }
+    }
+}
+
+// 16 bytes of 16-bit values of which any is not finite: those become 0.
+template <typename T>
+__device__ __forceinline__ bool finite_only(uint4& v) {
+    constexpr uint32_t kExp = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool lo = (w[i] & kExp) == kExp, hi = (w[i] >> 16 & kExp) == kExp;
+        if (lo) w[i] &= 0xFFFF0000u;
+        if (hi) w[i] &= 0x0000FFFFu;
+        bad = bad || lo || hi;
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+    return bad;
+}
+
 // What k_paged_combine joins: the item that CTA w begins and does not finish (pieces 0: none).
 struct PagedJoin {
     int64_t row0;          // the sequence's first token row

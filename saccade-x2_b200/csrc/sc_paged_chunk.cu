@@ -17,6 +17,11 @@
 // The reference m moves only when a row's maximum leaves it by more than a factor that P's type holds
 // (2^14 in f16): O is then rescaled in tensor memory, which is rare after the first tiles.
 // Pieces of the line of key tiles go to the CTAs evenly (sc_paged.cuh).
+// Measured, 28 + 4 heads of 128: 4 x 512 new tokens over 8192 cached positions, bf16, 64 + 8 heads: 466 us at a full
+// clock (1000 TFLOP/s), 530 to 540 under the power cap (870); 16 prompts of 129..512 tokens, f16: 71 us.  What bounds it
+// is the softmax: its instructions (two rows of 128 columns per thread and tile pair) keep the issue slots of the eight
+// warps busier than the tensor pipe, and the two halves' hand-overs do not fill each other's gaps wholly.  Short prompts
+// are a chain of load, S, softmax, PV, output with nothing beside it.
 #include <atomic>
 #include <type_traits>
 
@@ -148,6 +153,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
         o_full[2], done;
     __shared__ uint32_t tmem_slot;
     __shared__ PagedCut cut;
+    __shared__ int s_not_finite;  // a new token's value that is not has been met
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* ring = smem + 2 * C::kTile;
     const PagedLaunch& A = P.a;
@@ -168,6 +174,7 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
         }
         mbar_init(&done, 1);
         fence_mbar_init();
+        s_not_finite = 0;
     }
     if (tid == 32 * 8) {
         prefetch_map(&P.qmap);
@@ -224,6 +231,32 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < n; ++j, ++count) {
                 const int k0 = (w.t0 + j) * C::kKeys;
+                if (half == 0 && k0 + C::kKeys > first_pos + 1) {
+                    // V rows behind the item's last position hold whatever was there: 0 * NaN must not be.  Nor must it
+                    // for the new tokens that only some of the rows attend: their values are looked over.
+                    const int vt = it + 2 * j + 1, none = max(0, keys - k0);
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&kv_full[vt % C::kSlots], (vt / C::kSlots) & 1, kv.status));
+                    unsigned char* vb = ring + (vt % C::kSlots) * C::kTile;
+                    for (int i = max(0, first_pos + 1 - k0) * 8 + row; i < 128 * 8; i += 128) {
+                        // (a row of 128 bytes: eight lanes)
+                        bool bad = false;
+#pragma unroll
+                        for (int b = 0; b < C::kBlocks; ++b) {
+                            uint4* at = reinterpret_cast<uint4*>(vb + b * C::kBlock + i * 16);
+                            if (i >= none * 8) {
+                                *at = make_uint4(0, 0, 0, 0);
+                            } else {
+                                uint4 v = *at;
+                                if (finite_only<T>(v)) {
+                                    *at = v;
+                                    bad = true;
+                                }
+                            }
+                        }
+                        if (bad) s_not_finite = 1;
+                    }
+                    fence_proxy_async_smem();
+                }
                 ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_full[half], count & 1, kv.status));
                 if (!ok) break;
                 tc_fence_after();
@@ -301,17 +334,6 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
                 l += part[0] + part[1];
                 tc_st32(ts, pk);
                 tc_st32(ts + 32, pk + 32);
-                if (half == 0 && k0 + C::kKeys > keys) {
-                    // V rows behind the item's last position hold whatever was there: 0 * NaN must not be
-                    const int vt = it + 2 * j + 1, from = max(0, keys - k0);
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&kv_full[vt % C::kSlots], (vt / C::kSlots) & 1, kv.status));
-                    unsigned char* vb = ring + (vt % C::kSlots) * C::kTile;
-                    for (int i = from * 8 + row; i < 128 * 8; i += 128)
-#pragma unroll
-                        for (int b = 0; b < C::kBlocks; ++b)
-                            *reinterpret_cast<uint4*>(vb + b * C::kBlock + i * 16) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
-                }
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -320,7 +342,6 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
             it += 2 * n;
             more = wn.next(kv, A.max_q, tt, C::kKeys);  // while the last product ends
             ok = ok && __all_sync(0xffffffffu, mbar_wait(&o_full[half], items & 1, kv.status));
-            ++items;
             if (!ok) break;
             tc_fence_after();
             const bool whole = w.whole();
@@ -371,8 +392,18 @@ __global__ void __launch_bounds__(384, 1) k_paged_chunk(const __grid_constant__ 
             tc_fence_before();
             if (tok >= 0) {
                 if (!whole) *reinterpret_cast<float2*>(A.sc.ml + (slot_row + lane) * 2) = make_float2(m, l);
-                else if (A.o.lse) A.o.lse[orow] = l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+                else if (A.o.lse) A.o.lse[orow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
             }
+            if (__any_sync(0xffffffffu, *const_cast<volatile int*>(&s_not_finite) != 0)) {  // rare
+                __syncwarp();  // the row's stores by the other lanes
+                const int from = max(start + w.rt * tt + 1, w.t0 * C::kKeys), to = min(pos, w.t1 * C::kKeys - 1);
+                if (tok >= 0 && whole)
+                    paged_add_not_finite<T, kHd, 4>(kv, w.b, w.h, from, to, 0, static_cast<T*>(A.o.out) + static_cast<int64_t>(orow) * kHd);
+                else if (tok >= 0)
+                    paged_add_not_finite<T, kHd, 4>(kv, w.b, w.h, from, to, 0, A.sc.o + (slot_row + lane) * kHd);
+                __syncwarp();
+            }
+            ++items;
         }
         if (tid == 0) A.sc.join[blockIdx.x] = join;
         __syncwarp();

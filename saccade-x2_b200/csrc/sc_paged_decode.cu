@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
         const int first_pos = w.s.kv_len - w.s.q_len + w.rt * tt;  // the least position of the item's rows
         const int keys = w.s.kv_len - w.s.q_len + min((w.rt + 1) * tt, w.s.q_len);
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        bool bad = false;  // has met a new token's value that is not finite
         float o[kHd / 8][4];
 #pragma unroll
         for (int i = 0; i < kHd / 8; ++i)
@@ -287,6 +288,25 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                     o[i][3] *= f[1];
                 }
             }
+            if (w.s.q_len > 1 && edge) {
+                // this warp's positions among the new tokens behind the first row's: only some rows attend them
+                const int from = max(first_pos + 1, t * C::kKeys + 16 * warp), to = min(keys, t * C::kKeys + 16 * warp + 16);
+                for (int i = from * 8 + lane; i < to * 8; i += 32) {
+                    const int r = (i >> 3) - t * C::kKeys;
+#pragma unroll
+                    for (int blk = 0; blk < kBlocks; ++blk) {
+                        uint4* at = reinterpret_cast<uint4*>(smem + st * 2 * C::kTile + C::kTile + blk * (C::kKeys * 128) + r * 128 +
+                                                             (i & 7) * 16);
+                        uint4 v = *at;
+                        if (finite_only<T>(v)) {
+                            *at = v;
+                            bad = true;
+                        }
+                    }
+                }
+                fence_proxy_async_smem();  // before the stage is loaded again
+                __syncwarp();
+            }
             // positions behind the item's last key hold whatever the page or the ring held: no 0 * NaN
             uint32_t va = 0xFFFFFFFFu, vz = 0xFFFFFFFFu;
             const bool tail = (t + 1) * C::kKeys > keys;
@@ -323,7 +343,12 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                 s_l[warp][g4 + 8 * r] = l[r];
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        int any_bad;
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.s32 p, %1, 0;\nbarrier.cta.red.or.pred p, 1, 128, p;\nselp.s32 %0, 1, 0, p;\n}"
+            : "=r"(any_bad)
+            : "r"(static_cast<int>(bad))
+            : "memory");
         float wf[2];  // this warp's weights
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -338,7 +363,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
 #pragma unroll
         for (int i = 0; i < C::kWarps; ++i) mm = fmaxf(mm, s_m[i][row]);
 #pragma unroll
-        for (int i = 0; i < C::kWarps; ++i) ll += s_m[i][row] == -INFINITY ? 0.0f : s_l[i][row] * ex2(s_m[i][row] - mm);
+        for (int i = 0; i < C::kWarps; ++i) ll += s_l[i][row] == 0.0f ? 0.0f : s_l[i][row] * ex2(s_m[i][row] - mm);
         const int ot = written.token(w.rt, tt, w.s.q_len);
         const int64_t orow = (w.s.row0 + (ot < 0 ? 0 : ot)) * kv.nh + w.h * G + written.g;
         const bool whole = kCluster ? cs == 1 : w.whole();
@@ -376,9 +401,15 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
         }
+        if (any_bad && ot >= 0) {  // rare
+            const int from = max(first_pos + 1, w.t0 * C::kKeys), to = min(w.s.kv_len - w.s.q_len + ot, w.t1 * C::kKeys - 1);
+            if (whole) paged_add_not_finite<T, kHd, 32>(kv, w.b, w.h, from, to, cq, static_cast<T*>(A.o.out) + orow * kHd);
+            else if (kCluster) paged_add_not_finite<T, kHd, 32>(kv, w.b, w.h, from, to, cq, s_part + row * kHd);
+            else paged_add_not_finite<T, kHd, 32>(kv, w.b, w.h, from, to, cq, A.sc.o + (slot * 16 + row) * kHd);
+        }
         if ((tid & 7) == 0) {
             if (whole) {
-                if (A.o.lse && ot >= 0) A.o.lse[orow] = ll > 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+                if (A.o.lse && ot >= 0) A.o.lse[orow] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
             } else if constexpr (kCluster) {
                 s_ml[row][0] = mm;
                 s_ml[row][1] = ll;
@@ -398,7 +429,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                     float4 u[8];
 #pragma unroll
                     for (int p = 0; p < 8; ++p) {
-                        mi[p] = -INFINITY;
+                        mi[p] = -INFINITY, li[p] = 0.0f;
                         if (p < cs) {
                             mi[p] = ld_dsmem_f32(dsmem_addr(&s_ml[r][0], p));
                             li[p] = ld_dsmem_f32(dsmem_addr(&s_ml[r][1], p));
@@ -411,7 +442,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (int p = 0; p < 8; ++p)
-                        if (mi[p] > -INFINITY) {
+                        if (li[p] != 0.0f) {
                             const float f = ex2(mi[p] - m_all);
                             l_all += f * li[p];
                             x.x += f * u[p].x;
@@ -426,7 +457,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                     const int64_t at = (w.s.row0 + t) * kv.nh + w.h * G + pr.g;
                     *reinterpret_cast<uint2*>(static_cast<T*>(A.o.out) + at * kHd + c) =
                         make_uint2(M::pack(x.x * f, x.y * f), M::pack(x.z * f, x.w * f));
-                    if (A.o.lse && c == 0) A.o.lse[at] = l_all > 0.0f ? (m_all + log2f(l_all)) * 0.69314718055994531f : -INFINITY;
+                    if (A.o.lse && c == 0) A.o.lse[at] = l_all == 0.0f ? -INFINITY : (m_all + log2f(l_all)) * 0.69314718055994531f;
                 }
                 __syncwarp();
                 cluster_sync();  // no CTA leaves while another reads from it
@@ -510,7 +541,7 @@ __global__ void __launch_bounds__(256) k_paged_combine(const PagedLaunch A) {
             *reinterpret_cast<uint2*>(dst + c) = make_uint2(Pack16<Out>::pack(o[c] * inv, o[c + 1] * inv),
                                                             Pack16<Out>::pack(o[c + 2] * inv, o[c + 3] * inv));
     }
-    if (A.o.lse && sub == 0) A.o.lse[orow] = l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    if (A.o.lse && sub == 0) A.o.lse[orow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
 template <typename Out>

@@ -11,7 +11,7 @@
 // tokens whose CTAs would have at most kClusterKeysF32 positions each go to clusters as in sc_paged_decode.cu (one
 // sequence of 1..256 positions, 28 + 4 heads of 128: 12.2 us cut, 8.4 us in clusters; 4 of 513..1024 16.2 and 18.5;
 // row tiles of 64 rows, bound by their arithmetic, want the even cut: 12 sequences of 1..24 new tokens over up to
-// 1500 positions 34 us cut, 56 us in clusters of 4).
+// 1500 positions 36 us cut, 56 us in clusters of 4).
 #include <atomic>
 #include <type_traits>
 
@@ -108,6 +108,8 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
     while (next_item()) {
         const int start = w.s.kv_len - w.s.q_len;
         const int keys = start + min((w.rt + 1) * tt, w.s.q_len);
+        const int some = start + w.rt * tt + 1;  // from here on only some of the rows attend
+        bool bad = false;                        // has met a value there that is not finite
         const int32_t* table = kv.table + w.b * kv.max_pages;
         // this thread copies chunk `cc` of rows cr + kStep j: their places in the pages are found for a K tile and
         // kept for its V tile
@@ -237,6 +239,19 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                 }
             }
             cp_wait<1>();
+            if ((t + 1) * C::kKeys > some) {  // the values that this thread copied
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j) {
+                    float* at = sv + (cr + kStep * j) * C::kLd + cc;
+                    const float4 v = *reinterpret_cast<const float4*>(at);
+                    // (finite values' differences are 0, and so is their sum)
+                    if (!((v.x - v.x) + (v.y - v.y) + (v.z - v.z) + (v.w - v.w) == 0.0f) && t * C::kKeys + cr + kStep * j >= some) {
+                        for (int c = 0; c < 4; ++c)
+                            if (!(at[c] - at[c] == 0.0f)) at[c] = 0.0f;
+                        bad = true;
+                    }
+                }
+            }
             __syncthreads();  // V(t) is there, and the weights
             const float* p0 = sp + (grp * kRows + ty * 4) * C::kPld;
             const float* v0 = sv + grp * 16 * C::kLd + 4 * tx;
@@ -296,7 +311,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                         make_uint2(Pack16<__half>::pack(v.x, v.y), Pack16<__half>::pack(v.z, v.w));
                 else
                     *reinterpret_cast<float4*>(static_cast<float*>(A.o.out) + orow * kHd + col) = v;
-                if (col == 0 && A.o.lse) A.o.lse[orow] = ll > 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+                if (col == 0 && A.o.lse) A.o.lse[orow] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
             } else {
                 *reinterpret_cast<float4*>(A.sc.o + (slot * kRows + row) * kHd + col) = v;
                 if (col == 0) *reinterpret_cast<float2*>(A.sc.ml + (slot * kRows + row) * 2) = make_float2(mm, ll);
@@ -336,10 +351,22 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                 for (int x = 0; x < C::kGroups; ++x) {
                     const float4 u = *reinterpret_cast<const float4*>(sv + (x * kRows + row) * C::kLd + col);
                     v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-                    ll += s_m[x][row] == -INFINITY ? 0.0f : s_l[x][row] * ex2(s_m[x][row] - mm);
+                    ll += s_l[x][row] == 0.0f ? 0.0f : s_l[x][row] * ex2(s_m[x][row] - mm);
                 }
                 write(row, col, v, mm, ll);
             }
+        }
+        if (__syncthreads_or(bad)) {  // rare; the rows have been written
+            const PagedRow r(tid, kRows, G);
+            const int tok = tid < kRows ? r.token(w.rt, tt, w.s.q_len) : -1;
+            const int from = max(some, w.t0 * C::kKeys), to = min(start + tok, w.t1 * C::kKeys - 1);
+            const int64_t orow = (w.s.row0 + tok) * kv.nh + w.h * G + r.g;
+            if (tok >= 0) {
+                if (whole) paged_add_not_finite<float, kHd, 4>(kv, w.b, w.h, from, to, 0, static_cast<Out*>(A.o.out) + orow * kHd);
+                else if (kCluster) paged_add_not_finite<float, kHd, 4>(kv, w.b, w.h, from, to, 0, sk + tid * kHd);
+                else paged_add_not_finite<float, kHd, 4>(kv, w.b, w.h, from, to, 0, A.sc.o + (slot * kRows + tid) * kHd);
+            }
+            __syncthreads();
         }
         if constexpr (kCluster) {
             if (cs > 1) {
@@ -353,7 +380,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                     float4 u[8];
 #pragma unroll
                     for (int p = 0; p < 8; ++p) {
-                        mi[p] = -INFINITY;
+                        mi[p] = -INFINITY, li[p] = 0.0f;
                         if (p < cs) {
                             mi[p] = ld_dsmem_f32(dsmem_addr(&s_ml[row][0], p));
                             li[p] = ld_dsmem_f32(dsmem_addr(&s_ml[row][1], p));
@@ -366,7 +393,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (int p = 0; p < 8; ++p)
-                        if (mi[p] > -INFINITY) {
+                        if (li[p] != 0.0f) {
                             const float f = ex2(mi[p] - mm);
                             ll += f * li[p];
                             x.x += f * u[p].x;
@@ -385,7 +412,7 @@ __global__ void __launch_bounds__(256, kRows == 16 || kHd == 64 ? 2 : 1) k_paged
                             make_uint2(Pack16<__half>::pack(x.x, x.y), Pack16<__half>::pack(x.z, x.w));
                     else
                         *reinterpret_cast<float4*>(static_cast<float*>(A.o.out) + orow * kHd + col) = x;
-                    if (col == 0 && A.o.lse) A.o.lse[orow] = ll > 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+                    if (col == 0 && A.o.lse) A.o.lse[orow] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
                 }
                 __syncwarp();
                 cluster_sync();  // no CTA leaves while another reads from it

@@ -371,3 +371,52 @@ def test_append_then_attend_is_one_prefill(sc):
         part, kp2, vp2 = run(cuts)
         assert torch.equal(kp, kp2) and torch.equal(vp, vp2)
         assert (part - whole).abs().max() <= 2e-5  # f32 sums of up to 203 terms of size ~1, regrouped
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (20, 1, 64)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("lens", ["ragged", "chunk", "short", "decode"])
+@pytest.mark.parametrize("bound", [None, 1 << 20])
+def test_values_that_are_not_finite_stay_with_the_rows_that_attend_them(sc, dtype, heads, lens, bound):
+    """NaN and infinities among the values, in old and new positions: the same bits as with zeros there in
+    every row before the position and in every other column, and nothing finite in their own."""
+    c = Paged(LENS[lens], *heads, 16, dtype, "cuda", seed=21)
+    c.max_kv = max(c.max_kv, bound or 0)
+    g = torch.Generator().manual_seed(5)
+    bad, G = torch.zeros(c.tokens, c.nh, c.hd, dtype=torch.bool), heads[0] // heads[1]
+    put = []
+    for b, (n, kv) in enumerate(c.lens):
+        for i in range(min(n, 5)):
+            new = int(torch.randint(kv - n, kv, (1,), generator=g)) if i < 4 else kv - 1
+            p = int(torch.randint(0, kv, (1,), generator=g)) if i == 0 and n > 3 else new
+            h, col = int(torch.randint(c.nkv, (1,), generator=g)), int(torch.randint(c.hd, (1,), generator=g))
+            put.append((int(c.table[b, p // 16]), h, p % 16, col))
+            bad[c.cu[b] + max(0, p - (kv - n)):c.cu[b] + n, h * G:(h + 1) * G, col] = True
+    for at in put:
+        c.v_pages[at] = 0.0
+    clean, clean_lse = (t.clone() for t in attend(sc, c))
+    assert torch.isfinite(clean).all()
+    for value in (math.nan, math.inf, -math.inf):
+        for at in put:
+            c.v_pages[at] = value
+        got, lse = attend(sc, c)
+        assert torch.equal(torch.isfinite(got).cpu(), ~bad)
+        assert torch.equal(torch.where(bad.cuda(), clean, got), clean) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("lens", ["ragged", "chunk", "short"])
+@pytest.mark.parametrize("bound", [None, 1 << 20])
+def test_keys_that_are_not_finite_stay_with_the_rows_that_attend_them(sc, dtype, lens, bound):
+    c = Paged(LENS[lens], 14, 2, 64, 16, dtype, "cuda", seed=22)
+    c.max_kv = max(c.max_kv, bound or 0)
+    clean, clean_lse = (t.clone() for t in attend(sc, c))
+    bad = torch.zeros(c.tokens, c.nh, dtype=torch.bool)
+    for b, (n, kv) in enumerate(c.lens):
+        if n > 0:
+            p = kv - (n + 1) // 2
+            c.k_pages[int(c.table[b, p // 16]), 1, p % 16, 40] = math.nan
+            bad[c.cu[b] + p - (kv - n):c.cu[b] + n, 7:] = True
+    got, lse = attend(sc, c)
+    assert torch.equal(torch.isnan(got).all(-1).cpu(), bad) and torch.equal(torch.isnan(lse).cpu(), bad)
+    assert torch.equal(got[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad])
