@@ -11,8 +11,8 @@
 // word per token, so nothing of vocabulary size ever goes to global memory; every CTA of a row goes over
 // the row's whole history (a few KB from L2, tiles x 4 bytes per id) and counts its own tokens with integer
 // atomics, whose order does not matter.  (Thread-block clusters that read the history once and count into each
-// other's shared memory measured slower: 39 us against 21 at 64 x 152064 f32 with 768 ids, two cluster barriers
-// and 31 clusters of 16 at a time.)
+// other's shared memory measured slower: 39 us against 25 at 64 x 152064 f32 with 768 ids, two cluster barriers
+// and 31 clusters of 16 at a time.  So did CTAs that stay, with warps of their own for the counts: 44 us.)
 //   word = (bias entry + 1) << 20 | n << 1 | in the prompt
 // Few tokens are touched, but nearly every warp of a streaming pass would meet one and take its division along, so
 // whoever counts a token first sets its bit in a map of the tile, the map's tokens are listed and processed by
