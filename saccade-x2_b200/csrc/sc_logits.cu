@@ -15,10 +15,17 @@
 // and 31 clusters of 16 at a time.  So did CTAs that stay, with warps of their own for the counts: 44 us.)
 //   word = (bias entry + 1) << 20 | n << 1 | in the prompt
 // Few tokens are touched, but nearly every warp of a streaming pass would meet one and take its division along, so
-// whoever counts a token first sets its bit in a map of the tile, the map's tokens are listed and processed by
-// themselves, their words replaced by the values, and the streaming pass looks at a vector's bits only.
+// whoever changes a word first lists its token; the listed tokens are processed by themselves, a thread each, their
+// words replaced by the values, and the streaming pass takes what its vectors' words hold.  (Where the list overflows,
+// every word of the tile is looked at.)  A map of a bit per token in place of the words' look-up, and the list made from
+// it by prefix sums, measured 5.05 / 25.6 / 30.0 us on the three cases below; places in the list by warp ballots
+// 5.2 / 26.0 / 31.3.
 // Each CTA issues the loads of its first logits before it counts, so that they arrive meanwhile.  The best of
 // each tile goes to the scratch, and a second small kernel picks each row's.
+// Measured with everything on: 1 x 151936 f32, 256 ids 4.65 us; 64 x 152064 f32, up to 768 ids 24.5 us (3.2 TB/s; the
+// copy alone 13.4); 200 x 38017 bf16, up to 8000 ids 30.4 us (1 TB/s; the copy alone 8.3).  What bounds the last
+// two is the counting, a chain of short phases (zeroes, ids, atomics, list, division) in each of a few CTAs per SM; five,
+// six or eight smaller CTAs per SM read the ids more often: 33 to 37 us.
 #include <atomic>
 #include <string>
 
@@ -31,9 +38,8 @@ namespace sc {
 constexpr int kLogitThreads = 256;
 constexpr int kLogitWords = 10240;        // tokens of a tile at most (40 KB of words: four CTAs per SM)
 constexpr int kLogitMinTile = 2048;
-constexpr int kLogitMap = (kLogitWords + 16) / 32 + 1;
 constexpr int kLogitList = 1024;
-static_assert(kLogitMap <= 2 * kLogitThreads, "two words of the map per thread");
+constexpr uint32_t kLogitDone = 0x7FC0DEADu;  // a processed value's flipped bits (a NaN's, which becomes another), so that no word is 0
 constexpr int kLogitBatch = 6;            // 16-byte loads a thread has in flight
 constexpr int64_t kLogitMaxHistory = (1 << 19) - 1;  // 19 bits of a word count occurrences
 constexpr int64_t kLogitMaxRows = 1 << 20;
@@ -115,9 +121,8 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
     constexpr int kVec = LogitIo<T>::kVec;
     extern __shared__ __align__(16) uint32_t words[];  // one per token of the tile, from its first vector on
     __shared__ uint64_t s_best[kLogitThreads / 32];
-    __shared__ uint32_t s_map[kLogitMap];  // the tile's touched tokens
-    __shared__ uint16_t s_list[kLogitList];
-    __shared__ int s_sums[kLogitThreads / 32];
+    __shared__ uint16_t s_list[kLogitList];  // the tile's touched tokens, if they are so few
+    __shared__ int s_count;                  // and how many there are
     pdl_launch_dependents();
     const uint32_t row32 = blockIdx.x / static_cast<uint32_t>(a.tiles);
     const int64_t row = row32;
@@ -186,14 +191,17 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
     if (touched) {
         for (int i = tid; i < nvec * (kVec / 4); i += kLogitThreads)
             reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i <= nvec * kVec / 32; i += kLogitThreads) s_map[i] = 0;
+        if (tid == 0) s_count = 0;
         __syncthreads();
+        auto push = [&](int at) {  // whoever changed the word first
+            const int place = atomicAdd(&s_count, 1);
+            if (place < kLogitList) s_list[place] = static_cast<uint16_t>(at);
+        };
         for (int i = tid; i < nb; i += kLogitThreads) {
             const int v = a.bias_ids[b0 + i];
             if (v >= first && v - first < len) {
                 const int at = v - first + lead;
-                atomicMax(&words[at], static_cast<uint32_t>(i + 1) << 20);
-                atomicOr(&s_map[at >> 5], 1u << (at & 31));
+                if (atomicMax(&words[at], static_cast<uint32_t>(i + 1) << 20) == 0) push(at);
             }
         }
         if (nb > 0) __syncthreads();  // an entry's number is settled before counts join it in the word
@@ -210,41 +218,23 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
             for (int k = 0; k < kIds; ++k) {
                 if (id[k] < first || id[k] - first >= len) continue;
                 const int at = id[k] - first + lead;
-                if (i0 + k * kLogitThreads < prompt) atomicOr(&words[at], 1u);
-                else atomicAdd(&words[at], 2u);
-                atomicOr(&s_map[at >> 5], 1u << (at & 31));
+                const bool in_prompt = i0 + k * kLogitThreads < prompt;
+                if ((in_prompt ? atomicOr(&words[at], 1u) : atomicAdd(&words[at], 2u)) == 0) push(at);
             }
         }
         __syncthreads();
-        // the map's tokens as a list (thread t has words 2 t and 2 t + 1), kLogitList at a time, one thread each
-        const int lane = tid & 31, warp = tid >> 5, last = nvec * kVec / 32;
-        uint64_t mine = (2 * tid <= last ? s_map[2 * tid] : 0u) |
-                        static_cast<uint64_t>(2 * tid + 1 <= last ? s_map[2 * tid + 1] : 0u) << 32;
-        int upto = __popcll(mine);  // inclusive prefix sum over the block
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
+        auto process = [&](int at) {
+            const uint32_t y = __float_as_uint(process_one(LogitIo<T>::get(xb[at]), words[at], rep, pres, freq, a.bias_vals + b0));
+            words[at] = y == kLogitDone ? 0x7FFFFFFFu ^ kLogitDone : y ^ kLogitDone;
+        };
+        const int total = s_count;
+        if (total <= kLogitList) {
+            for (int i = tid; i < total; i += kLogitThreads) process(s_list[i]);
+        } else {
+            for (int at = tid; at < nvec * kVec; at += kLogitThreads)
+                if (words[at]) process(at);
         }
-        if (lane == 31) s_sums[warp] = upto;
         __syncthreads();
-        int total = 0;
-#pragma unroll
-        for (int i = 0; i < kLogitThreads / 32; ++i) {
-            if (i < warp) upto += s_sums[i];
-            total += s_sums[i];
-        }
-        int place = upto - __popcll(mine);
-        for (int base = 0; base < total; base += kLogitList) {
-            for (; mine && place < base + kLogitList; mine &= mine - 1)
-                s_list[place++ - base] = static_cast<uint16_t>(64 * tid + __ffsll(static_cast<long long>(mine)) - 1);
-            __syncthreads();
-            for (int i = tid; i < min(total - base, kLogitList); i += kLogitThreads) {
-                const int at = s_list[i];
-                words[at] = __float_as_uint(process_one(LogitIo<T>::get(xb[at]), words[at], rep, pres, freq, a.bias_vals + b0));
-            }
-            __syncthreads();
-        }
     }
     const bool even = first >= lead && ((first - lead) & (kVec - 1)) == 0;  // no vector's bits reach into the next word
     auto mask_bits = [&](int j) {
@@ -283,11 +273,13 @@ __global__ void __launch_bounds__(kLogitThreads, 4) k_process_logits(const Logit
 #pragma unroll
             for (int k = 0; k < kVec; ++k) f[k] = LogitIo<T>::get(v[k]);
             if (touched) {
-                const uint32_t bits = (s_map[j * kVec >> 5] >> (j * kVec & 31)) & ((1u << kVec) - 1u);
-                if (bits) {
 #pragma unroll
-                    for (int k = 0; k < kVec; ++k)
-                        if (bits & (1u << k)) f[k] = __uint_as_float(words[j * kVec + k]);
+                for (int k = 0; k < kVec; k += 4) {
+                    const uint4 w = reinterpret_cast<const uint4*>(words)[(j * kVec + k) / 4];
+                    if (w.x) f[k] = __uint_as_float(w.x ^ kLogitDone);
+                    if (w.y) f[k + 1] = __uint_as_float(w.y ^ kLogitDone);
+                    if (w.z) f[k + 2] = __uint_as_float(w.z ^ kLogitDone);
+                    if (w.w) f[k + 3] = __uint_as_float(w.w ^ kLogitDone);
                 }
             }
             if (mask) {

@@ -202,3 +202,34 @@ def test_in_a_graph(sc):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, w))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("share", [0.05, 0.5, 1.0])
+def test_many_tokens_touched(sc, dtype, share):
+    """Any share of a row's tokens in its history or bias list, results of either zero, infinities and NaN of any
+    bits among them: exactly the formula's f32 roundings."""
+    g = torch.Generator().manual_seed(17)
+    vocab = 20011
+    x = torch.randn(2, vocab, generator=g).to(dtype)
+    x[:, 0::11], x[:, 1::11], x[:, 2::11], x[:, 3::11] = 0.5, 0.0, math.inf, -math.inf
+    x[:, 4::11] = -0.0
+    if dtype == F32:
+        x.view(torch.int32)[:, 5::11] = 0x7FC0DEAD
+    h = torch.stack([torch.randperm(vocab, generator=g) for _ in range(2)])[:, :int(share * vocab)].to(torch.int32)
+    n = torch.zeros(2, vocab).scatter_(1, h.long(), 1.0)
+    ids = torch.arange(5, 4000, dtype=torch.int32)
+    b = torch.randn(len(ids), generator=g)
+    half = torch.full((2,), 0.5, device="cuda")
+    out, best, value = sc.process_logits(
+        x.cuda(), history=h.cuda(), hist_len=torch.full((2,), h.shape[1], dtype=torch.int32, device="cuda"), frequency=half,
+        bias_ptr=torch.tensor([0, 0, len(ids)], dtype=torch.int32, device="cuda"), bias_ids=ids.cuda(), bias_vals=b.cuda(),
+        return_best=True)
+    want = x.float() - 0.5 * n
+    want[1, 5:4000] += b
+    want = want.to(dtype).cuda()
+    nan = want.isnan()
+    assert torch.equal(out.isnan(), nan)
+    bits = torch.int32 if dtype == F32 else torch.int16
+    assert torch.equal(out.view(bits)[~nan], want.view(bits)[~nan])
+    assert torch.equal(best, want.argmax(-1)) if dtype == F32 else torch.equal(best, want.float().argmax(-1))
