@@ -104,14 +104,19 @@ class PagedKVCache:
 
     def pages(self, slot: int) -> List[int]:
         """The slot's pages, in order."""
-        return list(self._pages[slot])
+        return list(self._pages[self._slot(slot)])
+
+    def _slot(self, slot: int) -> int:
+        if not 0 <= slot < self.max_seqs:
+            raise ValueError(f"slot {slot}: the cache has {self.max_seqs}")
+        return slot
 
     def reserve(self, slot: int, positions: int) -> None:
         """Gives the slot the pages that `positions` positions need (it keeps those it has); RuntimeError, and
         nothing changed, where not enough are free."""
         if positions < 0 or positions > self.max_positions:
             raise ValueError(f"{positions} positions: the cache is made for up to {self.max_positions}")
-        have = self._pages[slot]
+        have = self._pages[self._slot(slot)]
         need = -(-positions // self.page_size) - len(have)
         if need <= 0:
             return
@@ -125,7 +130,7 @@ class PagedKVCache:
 
     def release(self, slot: int) -> None:
         """Takes the slot's pages back (what they hold stays until another sequence writes them)."""
-        self._free.extend(reversed(self._pages[slot]))
+        self._free.extend(reversed(self._pages[self._slot(slot)]))
         self._pages[slot] = []
         self.kv_len[slot] = 0
 

@@ -198,3 +198,12 @@ def test_logit_rules_refuse():
     assert r.bias_ptr.tolist() == [0, 2, 2, 3] and r.bias_ids.tolist() == [4, 2, 9]
     ptr, ids, vals = r._bias_of(torch.tensor([2, 0]))
     assert ptr.tolist() == [0, 1, 3] and ids.tolist() == [9, 4, 2] and vals.tolist() == [-1.0, 1.0, 3.0]
+
+
+def test_cache_refuses_slots_it_does_not_have():
+    c = sc.PagedKVCache(1, 4, 16, 1, 64, max_seqs=2, max_positions=32, device="cpu")
+    for slot in (-1, 2):
+        for call in (lambda: c.reserve(slot, 5), lambda: c.release(slot), lambda: c.pages(slot)):
+            with pytest.raises(ValueError, match="slot"):
+                call()
+    assert c.free_pages == 4
