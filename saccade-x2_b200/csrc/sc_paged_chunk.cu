@@ -25,8 +25,9 @@
 // warps of 16 rows each 465 us, the same with S ahead in steps of 64 positions (N = 64 products) 570, a tensor-core warp
 // per half and P handed over in two parts 543, the halves' exponentials strictly in turn 521, a quarter of them as
 // polynomials on the FMA pipe 10 to 25 us more each time, row sums in place of maxima to tell when a reference
-// must move 467.  Prompts spend half their time between items: queries' loads, the first S, the outputs, and code that
-// the instruction cache no longer holds (unrolling the output loop costs 6 us).
+// must move 467.  Prompts spend half their time between items: queries' loads, the first S, the outputs.  Their loop
+// unrolled with its loads ahead costs 6 us more; a kernel a third shorter (rolled loops, compact waits) the same or 20 us more
+// on the first case.
 #include <atomic>
 #include <type_traits>
 
