@@ -97,6 +97,7 @@ class PagedKVCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(max_seqs)]
+        self.decoder = lambda: None  # a reference to the decoder that runs on the slots
 
     @property
     def free_pages(self) -> int:

@@ -33,6 +33,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import weakref
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional
 
@@ -629,7 +630,8 @@ class PagedDecoder:
     start() takes the prompts, reserves the pages of their tokens and runs them in passes of at most `chunk`
     tokens per sequence (long prompts in several passes, shorter ones beside them); step() decodes one
     token of every sequence, as a replay of one captured graph after capture().  The decoder owns the cache's
-    slots 0 .. batch - 1 while it runs; finish() gives their pages back."""
+    slots 0 .. batch - 1 from start() on, and no other decoder starts on that cache; finish() gives their pages
+    back (also after a start() that found too few)."""
 
     def __init__(self, model: Qwen2Model, batch: int, rules: Optional[LogitRules] = None):
         if model.cache is None:
@@ -682,10 +684,14 @@ class PagedDecoder:
         lens = [int(p.numel()) for p in prompts]
         if max(lens) > c.max_positions:
             raise ValueError(f"a prompt of {max(lens)} tokens: the cache is made for up to {c.max_positions}")
+        if c.decoder() not in (None, self):
+            raise RuntimeError("another decoder runs on this cache; its finish() gives the sequences back")
+        c.decoder = weakref.ref(self)
         self.stream.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.device(dev), torch.cuda.stream(self.stream):
             for b, n in enumerate(lens):
                 c.reserve(b, n)
+            for b, n in enumerate(lens):
                 self.history[b, :n] = prompts[b].to(dev, torch.int32)
             self.prompt_len.copy_(torch.tensor(lens, dtype=torch.int32))
             self.hist_len.copy_(self.prompt_len)
@@ -774,6 +780,9 @@ class PagedDecoder:
     def finish(self) -> None:
         """Gives the sequences' pages back, after the steps in flight."""
         self.stream.synchronize()
+        self.lengths = [0] * self.B
+        if self.cache.decoder() is not self:
+            return
         for b in range(self.B):
             self.cache.release(b)
-        self.lengths = [0] * self.B
+        self.cache.decoder = lambda: None

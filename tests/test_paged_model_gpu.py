@@ -173,3 +173,30 @@ def test_decoder_refusals(q2, ck):
         for _ in range(20):
             dec.step()  # position 48 needs a fourth page
     dec.finish()
+
+
+def test_one_decoder_at_a_time(q2, ck):
+    """A second decoder on the same cache is refused until the first has finished, and finishing one that does
+    not run takes nothing from the one that does; a start() without enough pages leaves the run as it was."""
+    ps = prompts([20, 7], ck.cfg.vocab, 6)
+    model = paged(q2, ck, torch.float16, slots=2, pages=5)
+    want = q2.PagedDecoder(model, 2)
+    tokens = want.generate(ps, 6, graph=False)
+    want.finish()
+    first, second = q2.PagedDecoder(model, 2), q2.PagedDecoder(model, 1)
+    got = [first.start(ps)]
+    with pytest.raises(RuntimeError, match="another decoder"):
+        second.start(ps[:1])
+    second.finish()
+    with pytest.raises(RuntimeError, match="pages wanted"):
+        first.start(prompts([150, 7], ck.cfg.vocab, 7))
+    for _ in range(5):
+        got.append(first.step().clone())
+        first.stream.synchronize()
+    assert torch.equal(torch.stack(got, 1), tokens)
+    first.finish()
+    assert model.cache.free_pages == 5
+    second.start(ps[:1])
+    del second  # a decoder that is gone holds nothing up
+    assert torch.equal(first.generate(ps, 3), tokens[:, :3])
+    first.finish()
