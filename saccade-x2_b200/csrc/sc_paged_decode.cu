@@ -14,7 +14,7 @@
 // by a second kernel.  Where no CTA's share can pass kClusterKeys positions, finding the cut and that kernel
 // cost more than they even out: each (sequence, KV head) then goes to a cluster of 1 to 8 CTAs, as many as keep the
 // launch within one wave, which divide its tiles and join them through distributed shared memory.
-// Measured, f16, 28 + 4 heads of 128: one sequence of 640 positions 10.0 us cut, 5.7 us in clusters of 8; 64 of
+// Measured, f16, 28 + 4 heads of 128: one sequence of 640 positions 10.0 us cut, 5.9 us in clusters of 8; 64 of
 // 513..768 26.0 and 19.4 us (4.4 TB/s); one of 8192 18.7 and 14.3, of 16384 23.9 and 24.4, of 30000 29.4 and 41.2;
 // 200 of 2048 139 and 126.  8 of 20001..32768, 64 + 8 heads, bf16, cut: 143 us (6.2 TB/s, 0.96 of a copy).
 #include <atomic>

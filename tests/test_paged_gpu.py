@@ -420,3 +420,25 @@ def test_keys_that_are_not_finite_stay_with_the_rows_that_attend_them(sc, dtype,
     got, lse = attend(sc, c)
     assert torch.equal(torch.isnan(got).all(-1).cpu(), bad) and torch.equal(torch.isnan(lse).cpu(), bad)
     assert torch.equal(got[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("q_len,bound", [(1, 512), (1, 1 << 20), (70, 512)])
+def test_pages_more_than_2_31_elements_apart(sc, dtype, q_len, bound):
+    """Attention and appending in a cache whose last pages lie behind 2^31 elements: the bits of a small cache."""
+    c = Paged([(q_len, 2100), (q_len, 190)], 14, 2, 64, 256, dtype, "cuda", seed=31)
+    size, apart = 2 * 256 * 64, 2 ** 31 // (c.pages - 2) // 8 * 8 + 8 * 1024
+    far = [torch.empty(apart * (c.pages - 1) + size, dtype=dtype, device="cuda").as_strided(
+        (c.pages, 2, 256, 64), (apart, 256 * 64, 64, 1)) for _ in range(2)]
+    assert apart * (c.pages - 2) > 2 ** 31
+    far[0].copy_(c.k_pages), far[1].copy_(c.v_pages)
+    cos, sin = tables(2200, 64, "cuda")
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(c.tokens, 2, 64, device="cuda", generator=g).to(dtype) for _ in range(2))
+    out = []
+    for kp, vp in ((c.k_pages, c.v_pages), far):
+        q = sc.paged_append(c.q, k, v, cos, sin, kp, vp, c.table, c.cu_q, c.kv_len)
+        out.append((q, *sc.paged_attention(q, kp, vp, c.table, c.cu_q, c.kv_len, q_len, bound, return_lse=True)))
+    assert all(torch.equal(a, b) for a, b in zip(*out)) and torch.isfinite(out[0][1]).all()
+    assert torch.equal(far[0].nan_to_num(7.0), c.k_pages.nan_to_num(7.0))
+    assert torch.equal(far[1].nan_to_num(7.0), c.v_pages.nan_to_num(7.0))
