@@ -7,8 +7,11 @@
 //                   128-byte swizzle) by TMA into a ring of stages, two CTAs per SM: ~190 KB in flight
 //   4 warps         each takes 16 of the tile's 64 positions with a running maximum and sum of its own,
 //                   so no warp waits for another until the item ends: S = Q K^T (registers), weights
-//                   p = 2^(s scale log2 e - m) in f32, split into a high and a low 16-bit part
-//                   (P V then has 22 bits of p in f16, 16 in bf16, at no time that shows), O += P V
+//                   p = 2^(s scale log2 e - m) <= 1 in f32, split into a high and a low 16-bit part at no time that
+//                   shows, O += P V.  bf16's parts have 16 bits of p.  f16's are those of 2^15 p, so that its short
+//                   exponent range lies below the largest weight: 22 bits down to p = 2^-18, below that steps of
+//                   2^-39 (unscaled, weights under 2^-25 were lost, and thousands of them add up); the factor is
+//                   exact and leaves O again where the warps are joined
 //   item end        the 4 warps' maxima, sums and outputs are joined through shared memory.
 // Long sequences: the work is cut evenly over the CTAs along the positions (sc_paged.cuh) and the pieces are joined
 // by a second kernel.  Where no CTA's share can pass kClusterKeys positions, finding the cut and that kernel
@@ -75,6 +78,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
     using C = DecCfg<kHd>;
     using M = Pack16<T>;
     constexpr int kSteps = kHd / 16, kBlocks = kHd / 64;
+    constexpr float kScale = std::is_same<T, __half>::value ? 32768.0f : 1.0f;  // of the weights in O
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages];
     __shared__ float s_m[C::kWarps][16], s_l[C::kWarps][16];
@@ -273,10 +277,10 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
                 for (int n = 0; n < 2; ++n) {
                     const float p0 = ex2(s[n][2 * r] - ms), p1 = ex2(s[n][2 * r + 1] - ms);
                     l[r] += p0 + p1;
-                    const uint32_t h = M::pack(p0, p1);
+                    const uint32_t h = M::pack(p0 * kScale, p1 * kScale);
                     const float2 u = M::unpack(h);
                     ph[r + 2 * n] = h;
-                    pl[r + 2 * n] = M::pack(p0 - u.x, p1 - u.y);
+                    pl[r + 2 * n] = M::pack(p0 * kScale - u.x, p1 * kScale - u.y);
                 }
             }
             if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(DecCfg<kHd>::kThreads, 2) k_paged_decode(const
             float mm = -INFINITY;
 #pragma unroll
             for (int i = 0; i < C::kWarps; ++i) mm = fmaxf(mm, s_m[i][g4 + 8 * r]);
-            wf[r] = m[r] == -INFINITY ? 0.0f : ex2(m[r] - mm);
+            wf[r] = m[r] == -INFINITY ? 0.0f : ex2(m[r] - mm) * (1.0f / kScale);
         }
         // the rows as they are written: thread (row tid / 8, columns 4 (tid % 8) .. + 3)
         const int row = tid >> 3, cq = (tid & 7) * 4;
