@@ -31,6 +31,7 @@ each step one CUDA graph as GreedyDecoder's.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import weakref
@@ -650,9 +651,22 @@ class PagedDecoder:
         self.raw = self.logits = None           # the last step's logits before and after the rules
         self.lengths = [0] * batch              # positions held, on the host
         self.graph = None
-        self.stream = torch.cuda.Stream(device=dev)
+        self.stream = torch.cuda.Stream(device=dev)  # every pass runs here, between the caller's work (_running)
         self._xchg = (torch.zeros(batch, 2, dtype=torch.float32, device=dev),
                       torch.zeros(model.world, batch, 2, dtype=torch.float32, device=dev)) if model.world > 1 else None
+
+    @contextlib.contextmanager
+    def _running(self):
+        """The decoder's stream as the current one: behind everything the caller's stream holds (the rules' next mask, a
+        read of the tokens before), and before everything that it takes next."""
+        dev = self.model.device
+        caller = torch.cuda.current_stream(dev)
+        self.stream.wait_stream(caller)
+        try:
+            with torch.cuda.device(dev), torch.cuda.stream(self.stream):
+                yield
+        finally:
+            caller.wait_stream(self.stream)
 
     def _choose(self, logits: torch.Tensor, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The rules applied to a step's logits of all sequences (or of `rows`), and the next tokens."""
@@ -687,8 +701,7 @@ class PagedDecoder:
         if c.decoder() not in (None, self):
             raise RuntimeError("another decoder runs on this cache; its finish() gives the sequences back")
         c.decoder = weakref.ref(self)
-        self.stream.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.device(dev), torch.cuda.stream(self.stream):
+        with self._running():
             for b, n in enumerate(lens):
                 c.reserve(b, n)
             for b, n in enumerate(lens):
@@ -738,7 +751,7 @@ class PagedDecoder:
     def capture(self) -> None:
         """Records a step as a CUDA graph, after one eager step that sizes its buffers; that step counts (it
         decodes a token)."""
-        with torch.cuda.device(self.model.device), torch.cuda.stream(self.stream):
+        with self._running():
             self._reserve_next()
             self._step()
             self.lengths = [n + 1 for n in self.lengths]
@@ -753,8 +766,10 @@ class PagedDecoder:
         flush_deferred()
 
     def step(self) -> torch.Tensor:
-        """One decode step on the decoder's stream: the sequences' next tokens [batch] (device)."""
-        with torch.cuda.device(self.model.device), torch.cuda.stream(self.stream):
+        """One decode step: the sequences' next tokens [batch] (device; the next step writes them there again).  It runs
+        behind the work on the caller's current stream and before what that stream is given next, without
+        synchronising the host."""
+        with self._running():
             self._reserve_next()
             if self.graph is not None:
                 self.graph.replay()
@@ -771,10 +786,7 @@ class PagedDecoder:
             self.capture()
             out.append(self.ids.clone())
         while len(out) < steps:
-            self.step()
-            self.stream.synchronize()
-            out.append(self.ids.clone())
-        torch.cuda.current_stream(self.model.device).wait_stream(self.stream)
+            out.append(self.step().clone())
         return torch.stack(out[:steps], dim=1)
 
     def finish(self) -> None:
