@@ -73,7 +73,8 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 class _Workspaces:
     """Zero-filled workspaces keyed by (device, stream); grown on demand.  A replaced workspace is
-    kept alive: a CUDA graph captured with it still writes there when replayed."""
+    kept alive: a CUDA graph captured with it still writes there when replayed.  Each is at least half as large
+    again as the one before, so that all that are kept are together at most twice the newest."""
 
     def __init__(self):
         self._ws = {}
@@ -85,6 +86,7 @@ class _Workspaces:
         if ws is None or ws.numel() < nbytes:
             if ws is not None:
                 self._retired.append(ws)
+                nbytes = max(nbytes, ws.numel() + ws.numel() // 2)
             ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
             self._ws[key] = ws
         return ws
