@@ -271,6 +271,12 @@ class Qwen2Model:
         torch.backends.cuda.matmul.allow_tf32 = False
 
     # -------------------------------------------------------------- buffers
+    # A pass over the contiguous cache keeps its activations under their token counts, of which a run has two (the
+    # prompts' and the step's).  Ragged passes hardly ever repeat a count, and may run on several streams: theirs are
+    # torch's, given back at the pass's end in the order of its stream (a captured step holds its own).
+    def _fresh(self, key, shape, dtype):
+        return torch.empty(shape, dtype=dtype, device=self.device)
+
     def _buf(self, key, shape, dtype):
         b = self._bufs.get(key)
         if b is None or b.shape != torch.Size(shape) or b.dtype != dtype:
@@ -279,11 +285,13 @@ class Qwen2Model:
         return b
 
     def _routing(self, key, group: SaccadeLinearGroup, n_layers: int, T: int, fuse: bool):
-        """The fused router's buffers for `group` at T tokens (shared by every layer: the stream
-        orders their uses), or None where the group routes by itself."""
-        k = ("route",) + key + (T,)
+        """The fused router's buffers for `group` at T tokens on the current stream (shared by every layer: the
+        stream orders their uses), or None where the group routes by itself (all but 9..64 tokens do)."""
+        if not fuse or not group.takes_routing(T):
+            return None
+        k = ("route",) + key + (T, torch.cuda.current_stream(self.device).cuda_stream)
         if k not in self._bufs:
-            self._bufs[k] = GroupRouting(n_layers, T, self.device) if fuse and group.takes_routing(T) else None
+            self._bufs[k] = GroupRouting(n_layers, T, self.device)
         return self._bufs[k]
 
     def _stream(self):
@@ -314,7 +322,7 @@ class Qwen2Model:
                                          slot.data_ptr(), pos.data_ptr(), T, self.nh, self.nkv, hd, self.max_pos,
                                          max_query_pos, scratch.data_ptr(), scratch.numel() * 4, a16.data_ptr(), st))
 
-        return self._forward(ids, last, attend, torch.float16)
+        return self._forward(ids, last, attend, torch.float16, self._buf)
 
     def forward_paged(self, ids: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
                       last: torch.Tensor, max_q_len: int, max_kv_len: int) -> torch.Tensor:
@@ -326,7 +334,7 @@ class Qwen2Model:
         if c is None:
             raise ValueError("forward_paged needs a model on a paged cache")
         T, hd = ids.numel(), self.cfg.head_dim
-        qr = self._buf(("qr", T), (T, self.nh, hd), c.dtype)
+        qr = self._fresh("qr", (T, self.nh, hd), c.dtype)
 
         def attend(li, q, k, v, a16, st):
             paged_append(q.view(T, self.nh, hd), k.view(T, self.nkv, hd), v.view(T, self.nkv, hd), self.cos, self.sin,
@@ -335,27 +343,28 @@ class Qwen2Model:
                             out=a16.view(T, self.nh, hd), status=c.status)
 
         # the linears read f16 or bf16 (rounded to f16 as they read it); an f32 cache's attention writes f16
-        return self._forward(ids, last, attend, torch.bfloat16 if c.dtype == torch.bfloat16 else torch.float16)
+        return self._forward(ids, last, attend, torch.bfloat16 if c.dtype == torch.bfloat16 else torch.float16, self._fresh)
 
-    def _forward(self, ids: torch.Tensor, last: torch.Tensor, attend, attn_dtype: torch.dtype) -> torch.Tensor:
-        """The layers around `attend(layer, q, k, v, out, stream)`, which rotates, appends and attends."""
+    def _forward(self, ids: torch.Tensor, last: torch.Tensor, attend, attn_dtype: torch.dtype, buf) -> torch.Tensor:
+        """The layers around `attend(layer, q, k, v, out, stream)`, which rotates, appends and attends; `buf(key,
+        shape, dtype)` gives the activations."""
         cfg, dev = self.cfg, self.device
         T = ids.numel()
         H, hd = cfg.hidden, cfg.head_dim
         st = self._stream()
-        resid = self._buf(("resid", T), (T, H), torch.float32)
+        resid = buf(("resid", T), (T, H), torch.float32)
         check(LIB.sc_qwen2_embed(ids.data_ptr(), T, self.embed.data_ptr(), cfg.vocab, H, resid.data_ptr(),
                                  self.status.data_ptr(), st))
-        x16 = self._buf(("x16", T), (T, H), torch.float16)
-        q = self._buf(("q", T), (T, self.nh * hd), torch.float32)
-        k = self._buf(("k", T), (T, self.nkv * hd), torch.float32)
-        v = self._buf(("v", T), (T, self.nkv * hd), torch.float32)
-        a16 = self._buf(("a16", T), (T, self.nh * hd), attn_dtype)
-        delta = self._buf(("delta", T), (T, H), torch.float32)
+        x16 = buf(("x16", T), (T, H), torch.float16)
+        q = buf(("q", T), (T, self.nh * hd), torch.float32)
+        k = buf(("k", T), (T, self.nkv * hd), torch.float32)
+        v = buf(("v", T), (T, self.nkv * hd), torch.float32)
+        a16 = buf(("a16", T), (T, self.nh * hd), attn_dtype)
+        delta = buf(("delta", T), (T, H), torch.float32)
         ni = self.i1 - self.i0
-        g16 = self._buf(("g16", T), (T, ni), torch.float16)
-        u16 = self._buf(("u16", T), (T, ni), torch.float16)
-        m16 = self._buf(("m16", T), (T, ni), torch.float16)
+        g16 = buf(("g16", T), (T, ni), torch.float16)
+        u16 = buf(("u16", T), (T, ni), torch.float16)
+        m16 = buf(("m16", T), (T, ni), torch.float16)
         have_delta = False
         L0 = self.layers[0]
         fuse_norm = self.fused_route in ("norm", "all")
@@ -376,7 +385,7 @@ class Qwen2Model:
                                                x16.data_ptr(), _lib.SC_F16, st))
                 L["qkv"].forward(x16, out_dtype=torch.float32, outs=[q, k, v], biases=L["bias"])
             attend(li, q, k, v, a16, st)
-            self._row_layer(L["o"], a16, delta, ("o", T))
+            self._row_layer(L["o"], a16, delta, ("o", T), buf)
             if r_gu is not None:
                 check(LIB.sc_qwen2_add_rmsnorm_route(resid.data_ptr(), delta.data_ptr(), L["norm_post"].data_ptr(), T,
                                                      H, eps, x16.data_ptr(), L["gateup"]._h, r_gu.mask_p, r_gu.ridx_p,
@@ -393,34 +402,34 @@ class Qwen2Model:
                 L["downg"].forward_routed(m16, r_down, out_dtype=torch.float32, outs=[delta])
             else:
                 check(LIB.sc_qwen2_silu_mul(g16.data_ptr(), u16.data_ptr(), T * ni, m16.data_ptr(), st))
-                self._row_layer(L["down"], m16, delta, ("down", T))
+                self._row_layer(L["down"], m16, delta, ("down", T), buf)
             have_delta = True
         nl = last.numel()
-        rl = self._buf(("rlast", nl), (nl, H), torch.float32)
-        dl = self._buf(("dlast", nl), (nl, H), torch.float32)
+        rl = buf(("rlast", nl), (nl, H), torch.float32)
+        dl = buf(("dlast", nl), (nl, H), torch.float32)
         torch.index_select(resid, 0, last, out=rl)
         torch.index_select(delta, 0, last, out=dl)
-        xn = self._buf(("xn", nl), (nl, H), torch.float32)
+        xn = buf(("xn", nl), (nl, H), torch.float32)
         check(LIB.sc_qwen2_add_rmsnorm(rl.data_ptr(), dl.data_ptr(), self.final_norm.data_ptr(), nl, H,
                                        ctypes.c_float(cfg.eps), xn.data_ptr(), _lib.SC_F32, st))
-        return self._lm_head(xn)
+        return self._lm_head(xn, buf)
 
-    def _row_layer(self, op: SaccadeLinearOp, x16: torch.Tensor, out_f32: torch.Tensor, key):
+    def _row_layer(self, op: SaccadeLinearOp, x16: torch.Tensor, out_f32: torch.Tensor, key, buf):
         """o / down: y = f32(f16(acc)) (model.rs:61) into out_f32; on several ranks the rank's f32 partial
         sums and router sums are all-reduced, then routed and rounded."""
         if self.world == 1:
             op.forward(x16, out_dtype=torch.float32, out=out_f32)
             return
         T = x16.shape[0]
-        part = self._buf(key + ("part",), (op.exchange_size(T),), torch.float32)
+        part = buf(key + ("part",), (op.exchange_size(T),), torch.float32)
         op.forward_split(x16, part)
         self._all_reduce(part)
         op.finalize_split(part, T, self.world, out=out_f32)
 
-    def _lm_head(self, xn: torch.Tensor) -> torch.Tensor:
+    def _lm_head(self, xn: torch.Tensor, buf) -> torch.Tensor:
         """logits = x . W^T with f16 W: x = hi + lo (f16 each), two f16 GEMMs with f32 accumulation."""
         nl = xn.shape[0]
-        hilo = self._buf(("hilo", nl), (2 * nl, xn.shape[1]), torch.float16)
+        hilo = buf(("hilo", nl), (2 * nl, xn.shape[1]), torch.float16)
         hi = xn.to(torch.float16)
         hilo[:nl].copy_(hi)
         hilo[nl:].copy_((xn - hi.float()).to(torch.float16))

@@ -138,3 +138,64 @@ def test_generate_keeps_each_steps_tokens(q2, ck):
         torch.cuda._sleep(BUSY)
         assert dec.generate(ps, 12, graph=graph).tolist() == want
         dec.finish()
+
+
+def test_ragged_passes_keep_no_memory(q2, ck):
+    """Passes of many different token counts, and decoders that come and go: what is allocated stays the same."""
+    dec = decoder(q2, ck, batch=4)
+    m, c = dec.model, dec.cache
+    for b in range(4):
+        c.reserve(b, 160)
+    kv = lambda t: torch.tensor([t], dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def one(t):
+        ids = torch.zeros(t, dtype=torch.int64, device="cuda")
+        m.forward_paged(ids, c.block_table[:1], torch.tensor([0, t], dtype=torch.int32, device="cuda"), kv(t),
+                        torch.tensor([t - 1], device="cuda"), t, t)
+
+    for t in (160, 1, 8, 9, 64, 65):
+        one(t)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for t in range(1, 161):
+        one(t)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+    for b in range(4):
+        c.release(b)
+    dec.generate(prompts([150, 150, 150, 150], ck.cfg.vocab, 1), 2)
+    dec.finish()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for i in range(12):
+        dec.generate(prompts([3 + 11 * i, 140 - 7 * i, 1 + i, 77], ck.cfg.vocab, i), 3)
+        dec.finish()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() <= before + 4 * 4 * ck.cfg.vocab * 4  # a step's logits, before and after the rules
+
+
+@pytest.mark.parametrize("graph", [True, False], ids=["graph", "eager"])
+def test_a_pass_on_another_stream_beside_the_decoder(q2, ck, graph):
+    """The model runs another sequence, of as many new tokens as the decoder's batch, on a stream that nothing orders
+    with the decoder's steps: both give what they give alone."""
+    ps = prompts([9, 20], ck.cfg.vocab, 1)
+    dec = decoder(q2, ck, no_repeats(2))
+    m, c = dec.model, dec.cache
+    want = dec.generate(ps, 25, graph=graph).tolist()
+    c.reserve(3, 2)
+    ids = torch.tensor([5, 6], device="cuda")
+    args = (ids, c.block_table[3:4], torch.tensor([0, 2], dtype=torch.int32, device="cuda"),
+            torch.tensor([2], dtype=torch.int32, device="cuda"), torch.tensor([0, 1], device="cuda"), 2, 2)
+    alone = m.forward_paged(*args).clone()
+    side, beside = torch.cuda.Stream(), []
+    got = [dec.start(ps).tolist()]
+    torch.cuda.synchronize()
+    for _ in range(24):
+        dec.step()
+        with torch.cuda.stream(side):
+            beside += [m.forward_paged(*args) for _ in range(2)]
+        got.append(dec.ids.tolist())
+    torch.cuda.synchronize()
+    assert [list(t) for t in zip(*got)] == want
+    assert all(torch.equal(x, alone) for x in beside)
+    dec.finish()
