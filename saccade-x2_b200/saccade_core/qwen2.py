@@ -638,7 +638,8 @@ class PagedDecoder:
     """Decodes a batch of ragged prompts on a model's paged cache, with LogitRules on every step's logits.
 
     start() takes the prompts, reserves the pages of their tokens and runs them in passes of at most `chunk`
-    tokens per sequence (long prompts in several passes, shorter ones beside them); step() decodes one
+    tokens per sequence and `max_tokens` in all (long prompts in several passes, shorter ones beside them, the rest
+    later: a pass's activations take memory by its tokens, 182 KB each at the 7B model); step() decodes one
     token of every sequence, as a replay of one captured graph after capture().  The decoder owns the cache's
     slots 0 .. batch - 1 from start() on, and no other decoder starts on that cache; finish() gives their pages
     back (also after a start() that found too few)."""
@@ -696,14 +697,14 @@ class PagedDecoder:
         self.hist_len[rows] += 1
         self.ids[rows] = tokens
 
-    def start(self, prompts, chunk: int = 2048) -> torch.Tensor:
+    def start(self, prompts, chunk: int = 2048, max_tokens: int = 32768) -> torch.Tensor:
         """Runs the prompts (a list of `batch` 1-D id tensors, each of at least one token) and returns the first
         tokens [batch]."""
         m, c, dev = self.model, self.cache, self.model.device
         if len(prompts) != self.B or any(p.dim() != 1 or p.numel() < 1 for p in prompts):
             raise ValueError(f"{self.B} prompts of at least one token are wanted")
-        if chunk < 1:
-            raise ValueError("chunk must be at least 1")
+        if chunk < 1 or max_tokens < 1:
+            raise ValueError("chunk and max_tokens must be at least 1")
         lens = [int(p.numel()) for p in prompts]
         if max(lens) > c.max_positions:
             raise ValueError(f"a prompt of {max(lens)} tokens: the cache is made for up to {c.max_positions}")
@@ -719,7 +720,12 @@ class PagedDecoder:
             self.hist_len.copy_(self.prompt_len)
             done = [0] * self.B
             while True:
-                part = [(b, done[b], min(lens[b], done[b] + chunk)) for b in range(self.B) if done[b] < lens[b]]
+                part, left = [], max_tokens
+                for b in range(self.B):
+                    n = min(chunk, lens[b] - done[b], left)
+                    if n > 0:
+                        part.append((b, done[b], done[b] + n))
+                        left -= n
                 if not part:
                     break
                 ids = torch.cat([prompts[b][i:j].to(dev, torch.int64) for b, i, j in part])
@@ -788,9 +794,10 @@ class PagedDecoder:
             self.lengths = [n + 1 for n in self.lengths]
         return self.ids
 
-    def generate(self, prompts, steps: int, *, chunk: int = 2048, graph: bool = True) -> torch.Tensor:
+    def generate(self, prompts, steps: int, *, chunk: int = 2048, max_tokens: int = 32768,
+                 graph: bool = True) -> torch.Tensor:
         """Tokens [batch, steps] after the prompts."""
-        out = [self.start(prompts, chunk)]
+        out = [self.start(prompts, chunk, max_tokens)]
         if graph and self.graph is None and steps > 1:
             self.capture()
             out.append(self.ids.clone())
