@@ -452,11 +452,19 @@ class Qwen2Model:
         return int(sum(int(L[n].undecided.item()) for L in self.layers for n in ("o", "down")))
 
     def check_device(self):
+        """Raises what the device has recorded: in a layer, in the paged cache's kernels, or a token id."""
         for L in self.layers:
             for name in PROJ:
                 L[name].check_device()
+        self.check_passes()
+
+    def check_passes(self):
+        """check_device() without the layers' own words: a synchronisation instead of one per layer."""
         if int(self.status[0].item()) != 0:
+            self.status.zero_()
             raise _lib.CTarqError(_lib.SC_EDEVICE, "a token id outside the vocabulary")
+        if self.cache is not None:
+            self.cache.check_device()
 
 
 # ------------------------------------------------------------------ calibration and generation
@@ -699,7 +707,8 @@ class PagedDecoder:
 
     def start(self, prompts, chunk: int = 2048, max_tokens: int = 32768) -> torch.Tensor:
         """Runs the prompts (a list of `batch` 1-D id tensors, each of at least one token) and returns the first
-        tokens [batch]."""
+        tokens [batch]; raises what the passes have recorded on the device (step() does not wait to see: the model's
+        check_passes() tells)."""
         m, c, dev = self.model, self.cache, self.model.device
         if len(prompts) != self.B or any(p.dim() != 1 or p.numel() < 1 for p in prompts):
             raise ValueError(f"{self.B} prompts of at least one token are wanted")
@@ -714,6 +723,7 @@ class PagedDecoder:
         with self._running():
             for b, n in enumerate(lens):
                 c.reserve(b, n)
+            self.lengths = [0] * self.B  # until the prompts have passed
             for b, n in enumerate(lens):
                 self.history[b, :n] = prompts[b].to(dev, torch.int32)
             self.prompt_len.copy_(torch.tensor(lens, dtype=torch.int32))
@@ -744,9 +754,9 @@ class PagedDecoder:
                 for b, _, j in part:
                     done[b] = j
             self.kv_len.copy_(self.prompt_len)
-            self.lengths = lens
             first = self.ids.clone()
-        self.stream.synchronize()
+        m.check_passes()
+        self.lengths = lens
         return first
 
     def _step(self) -> None:
@@ -803,6 +813,7 @@ class PagedDecoder:
             out.append(self.ids.clone())
         while len(out) < steps:
             out.append(self.step().clone())
+        self.model.check_passes()
         return torch.stack(out[:steps], dim=1)
 
     def finish(self) -> None:
