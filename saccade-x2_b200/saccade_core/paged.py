@@ -15,7 +15,8 @@ allocate nothing but their outputs and scratch (through torch's allocator) and d
 from __future__ import annotations
 
 import ctypes
-from typing import List, Optional
+import weakref
+from typing import List, Optional, Set
 
 import torch
 
@@ -98,6 +99,8 @@ class PagedKVCache:
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(max_seqs)]
         self.decoder = lambda: None  # a reference to the decoder that runs on the slots
+        self._claimed: Set[int] = set()  # the slots it has, and its stream
+        self._claimed_stream = None
 
     @property
     def free_pages(self) -> int:
@@ -122,6 +125,8 @@ class PagedKVCache:
         if need <= 0:
             return
         if need > len(self._free):
+            self._reclaim()
+        if need > len(self._free):
             raise RuntimeError(f"{need} pages wanted, {len(self._free)} of {self.num_pages} free")
         new = [self._free.pop() for _ in range(need)]
         row = torch.tensor(new, dtype=torch.int32).pin_memory() if self.device.type == "cuda" else torch.tensor(
@@ -134,6 +139,31 @@ class PagedKVCache:
         self._free.extend(reversed(self._pages[self._slot(slot)]))
         self._pages[slot] = []
         self.kv_len[slot] = 0
+        if self.decoder() is None:
+            self._claimed.discard(slot)
+
+    def claim(self, decoder, slots: int, stream) -> None:
+        """Slots 0 .. slots - 1 are `decoder`'s, which works on `stream`, until give_back(); RuntimeError where another
+        decoder has not given its slots back.  Those of one that is gone are released first."""
+        if self.decoder() not in (None, decoder):
+            raise RuntimeError("another decoder runs on this cache; its finish() gives the sequences back")
+        self._reclaim()
+        self.decoder, self._claimed, self._claimed_stream = weakref.ref(decoder), set(range(slots)), stream
+
+    def give_back(self, decoder) -> None:
+        """Releases the slots that `decoder` has claimed (its work on them has ended), if it has any."""
+        if self.decoder() is decoder:
+            self.decoder = lambda: None
+            for slot in sorted(self._claimed):
+                self.release(slot)
+
+    def _reclaim(self) -> None:
+        """Releases what a decoder has claimed that is gone without giving it back, after its last steps."""
+        if self._claimed and self.decoder() is None:
+            if self._claimed_stream is not None:
+                self._claimed_stream.synchronize()
+            for slot in sorted(self._claimed):
+                self.release(slot)
 
     def check_device(self) -> None:
         """Raises where a kernel met a position, page or length outside the tables (or a wait ran out)."""

@@ -34,7 +34,6 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
-import weakref
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional
 
@@ -650,7 +649,8 @@ class PagedDecoder:
     later: a pass's activations take memory by its tokens, 182 KB each at the 7B model); step() decodes one
     token of every sequence, as a replay of one captured graph after capture().  The decoder owns the cache's
     slots 0 .. batch - 1 from start() on, and no other decoder starts on that cache; finish() gives their pages
-    back (also after a start() that found too few)."""
+    back (also after a start() that found too few).  Those of a decoder that is dropped without it go back when the
+    next one starts, or when pages run short."""
 
     def __init__(self, model: Qwen2Model, batch: int, rules: Optional[LogitRules] = None):
         if model.cache is None:
@@ -717,9 +717,7 @@ class PagedDecoder:
         lens = [int(p.numel()) for p in prompts]
         if max(lens) > c.max_positions:
             raise ValueError(f"a prompt of {max(lens)} tokens: the cache is made for up to {c.max_positions}")
-        if c.decoder() not in (None, self):
-            raise RuntimeError("another decoder runs on this cache; its finish() gives the sequences back")
-        c.decoder = weakref.ref(self)
+        c.claim(self, self.B, self.stream)
         with self._running():
             for b, n in enumerate(lens):
                 c.reserve(b, n)
@@ -820,8 +818,4 @@ class PagedDecoder:
         """Gives the sequences' pages back, after the steps in flight."""
         self.stream.synchronize()
         self.lengths = [0] * self.B
-        if self.cache.decoder() is not self:
-            return
-        for b in range(self.B):
-            self.cache.release(b)
-        self.cache.decoder = lambda: None
+        self.cache.give_back(self)
