@@ -42,12 +42,14 @@ class LogitRules:
     """What a batch's logits go through: repetition, presence and frequency penalties (a number, or one per
     sequence), bias (one {token: value} per sequence) and grammar masks (int32 [masks, words], one bit per
     token; mask_row: each sequence's mask or -1).  The tensors stay where they are, so a captured step follows
-    what is written into them (a grammar's next mask, another penalty)."""
+    what is written into them (a grammar's next mask, another penalty).  The rules are of `batch` sequences."""
 
     def __init__(self, batch: int, device, *, repetition: Union[None, float, Sequence[float]] = None,
                  presence: Union[None, float, Sequence[float]] = None,
                  frequency: Union[None, float, Sequence[float]] = None, bias: Optional[Sequence[Dict[int, float]]] = None,
                  mask: Optional[torch.Tensor] = None, mask_row: Optional[Sequence[int]] = None):
+        self.batch = batch
+
         def floats(v, what):
             if v is None:
                 return None
@@ -72,8 +74,27 @@ class LogitRules:
             self.bias_ptr = torch.tensor(ptr, dtype=torch.int32, device=device)
             self.bias_ids = torch.tensor([t for b in bias for t in b], dtype=torch.int32, device=device)
             self.bias_vals = torch.tensor([x for b in bias for x in b.values()], dtype=torch.float32, device=device)
+        if mask is not None and (mask.dim() != 2 or mask.dtype != torch.int32 or not mask.is_contiguous()):
+            raise ValueError("mask must be a contiguous int32 tensor [masks, words]")
+        if mask_row is None:
+            if mask is not None and mask.shape[0] < batch:
+                raise ValueError(f"{mask.shape[0]} masks for {batch} sequences (mask_row names each one's)")
+        else:
+            mask_row = list(mask_row)
+            if mask is None or len(mask_row) != batch or max(mask_row, default=-1) >= mask.shape[0]:
+                raise ValueError("mask_row must be each sequence's mask, one of those of `mask`, or -1")
         self.mask = None if mask is None else mask.to(device)
-        self.mask_row = None if mask_row is None else torch.tensor(list(mask_row), dtype=torch.int32, device=device)
+        self.mask_row = None if mask_row is None else torch.tensor(mask_row, dtype=torch.int32, device=device)
+
+    def check(self, batch: int, device: torch.device, vocab: int) -> None:
+        """ValueError where these rules are not of `batch` sequences over a vocabulary of `vocab` tokens on `device`."""
+        if self.batch != batch:
+            raise ValueError(f"rules of {self.batch} sequences for {batch}")
+        tensors = (self.repetition, self.presence, self.frequency, self.bias_ptr, self.mask, self.mask_row)
+        if any(t is not None and t.device != device for t in tensors):
+            raise ValueError(f"the rules must be on {device}")
+        if self.mask is not None and self.mask.shape[1] * 32 < vocab:
+            raise ValueError(f"masks of {self.mask.shape[1]} words do not cover {vocab} tokens")
 
     def apply(self, logits: torch.Tensor, *, rows: Optional[torch.Tensor] = None, history=None, prompt_len=None,
               hist_len=None, vocab_begin: int = 0, out: Optional[torch.Tensor] = None,

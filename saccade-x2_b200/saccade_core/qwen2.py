@@ -658,6 +658,8 @@ class PagedDecoder:
         c, dev = model.cache, model.device
         if batch < 1 or batch > c.max_seqs:
             raise ValueError(f"batch must be 1..{c.max_seqs} (the cache's sequences)")
+        if rules is not None:
+            rules.check(batch, model.embed.device, model.cfg.vocab)
         self.model, self.B, self.cache, self.rules = model, batch, c, rules or LogitRules(batch, dev)
         self.ids = torch.zeros(batch, dtype=torch.int64, device=dev)
         self.history = torch.zeros(batch, c.max_positions + 1, dtype=torch.int32, device=dev)
