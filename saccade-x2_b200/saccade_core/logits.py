@@ -14,6 +14,8 @@ import torch
 
 from .paged import _serve  # bound to the library there
 
+MAX_HISTORY = 524287  # ids of a row's history (sc_qwen2_process_logits)
+
 
 def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
                    prompt_len: Optional[torch.Tensor] = None, hist_len: Optional[torch.Tensor] = None,
@@ -28,7 +30,7 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
       in the row's history:  x = x / repetition where x > 0, x * repetition elsewhere
       n times among its generated tokens:  x = x - frequency * n - (presence if n > 0)
       x = x + the token's (last) bias entry;  -inf where the row's mask does not allow the token
-    history int32 [rows, width]: the first hist_len[r] ids are row r's, the first prompt_len[r] of them its
+    history int32 [rows, width <= MAX_HISTORY]: the first hist_len[r] ids are row r's, the first prompt_len[r] of them its
     prompt (no prompt_len: all generated); ids of other tokens than the slice's are passed over.
     repetition (> 0), presence, frequency: f32 [rows].  bias_ids / bias_vals entries bias_ptr[r]..bias_ptr[r + 1]
     (int32 [rows + 1]) are row r's, at most 4095 of them.  mask int32 [masks, words]: bit v % 32 of word

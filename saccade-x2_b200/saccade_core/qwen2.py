@@ -44,7 +44,7 @@ from . import _lib
 from ._lib import LIB, check
 from .compress import ProfileRunner, compress_tensor_to_saccade, compute_percentile_threshold
 from .graph import no_gc
-from .logits import LogitRules
+from .logits import MAX_HISTORY, LogitRules
 from .paged import PagedKVCache, paged_append, paged_attention
 from .op import GroupRouting, SaccadeConfig, SaccadeLinearGroup, SaccadeLinearOp, SparseDeltaMatrix, flush_deferred
 
@@ -658,6 +658,8 @@ class PagedDecoder:
         c, dev = model.cache, model.device
         if batch < 1 or batch > c.max_seqs:
             raise ValueError(f"batch must be 1..{c.max_seqs} (the cache's sequences)")
+        if c.max_positions + 1 > MAX_HISTORY:
+            raise ValueError(f"a cache of {c.max_positions} positions: a decoder's history holds {MAX_HISTORY - 1}")
         if rules is not None:
             rules.check(batch, model.embed.device, model.cfg.vocab)
         self.model, self.B, self.cache, self.rules = model, batch, c, rules or LogitRules(batch, dev)
