@@ -767,6 +767,13 @@ class PagedDecoder:
                                           self.cache.max_positions)
         self._take(self.last, self._choose(logits))
 
+    def _eager_step(self) -> None:
+        try:
+            self._step()
+        except BaseException:
+            self.lengths = [0] * self.B  # it may have moved the sequences on: start() begins anew
+            raise
+
     def _reserve_next(self) -> None:
         if min(self.lengths) < 1:
             raise RuntimeError("start() takes the prompts first")
@@ -780,14 +787,18 @@ class PagedDecoder:
         decodes a token)."""
         with self._running():
             self._reserve_next()
-            self._step()
+            self._eager_step()
             self.lengths = [n + 1 for n in self.lengths]
         self.stream.synchronize()
         eager = self.raw, self.logits
-        self.graph = torch.cuda.CUDAGraph()
-        with no_gc(), torch.cuda.graph(self.graph, stream=self.stream):
-            self._step()
-        self._graph_logits = self.raw, self.logits  # written by every replay
+        graph = torch.cuda.CUDAGraph()
+        try:
+            with no_gc(), torch.cuda.graph(graph, stream=self.stream):
+                self._step()
+        except BaseException:
+            self.raw, self.logits = eager
+            raise
+        self.graph, self._graph_logits = graph, (self.raw, self.logits)  # written by every replay
         self.raw, self.logits = eager
         self.stream.synchronize()
         flush_deferred()
@@ -802,7 +813,7 @@ class PagedDecoder:
                 self.graph.replay()
                 self.raw, self.logits = self._graph_logits
             else:
-                self._step()
+                self._eager_step()
             self.lengths = [n + 1 for n in self.lengths]
         return self.ids
 
