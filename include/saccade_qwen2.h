@@ -116,7 +116,8 @@ SC_API sc_status sc_qwen2_silu_mul_route(const uint16_t* gate, const uint16_t* u
  * the rotated k and v into the pages and the rotated q to q_out [tokens][num_heads][head_dim], all as
  * cache_dtype with one rounding.  q, k, v: in_dtype rows (heads contiguous) q_stride, k_stride and
  * v_stride elements apart, so slices of one projection buffer serve.  in_dtype is SC_F32 or
- * cache_dtype.  q_out may be q itself (same type, q_stride = num_heads * head_dim).  A token whose
+ * cache_dtype.  q_out may be q itself (same type, q_stride = num_heads * head_dim) and must not lie over q, k or v
+ * otherwise.  A token whose
  * position lies outside the rotation tables is left out; one without a page gets its q only. */
 SC_API sc_status sc_qwen2_paged_append(const void* q, const void* k, const void* v, int in_dtype, int64_t q_stride,
                                        int64_t k_stride, int64_t v_stride, int64_t tokens, const float* cos_table,
@@ -135,7 +136,8 @@ SC_API size_t sc_qwen2_paged_attention_scratch(int64_t num_seqs, int num_heads, 
  * positions 0..p, o = sum softmax(scale * q . k) v per query head (grouped onto the KV heads), f32
  * sums and softmax statistics.  q [tokens][num_heads][head_dim] of cache_dtype, rows q_stride elements
  * apart; out [tokens][num_heads][head_dim] contiguous, out_dtype = cache_dtype (an f32 cache may also
- * write SC_F16, the linears' input).  lse (nullable, f32 [tokens][num_heads]) = log sum exp(scale * q . k).
+ * write SC_F16, the linears' input); it may be q itself (same type, q_stride = num_heads * head_dim), or none of its
+ * bytes.  lse (nullable, f32 [tokens][num_heads]) = log sum exp(scale * q . k).
  * A token at a negative position attends nothing: its output is 0, its lse -inf.  max_q_len and max_kv_len bound
  * every sequence's new tokens and positions and choose the kernels (a sequence with more new tokens is skipped and
  * recorded; more positions are attended all the same).  16-bit caches need q, the pages and their strides 16-byte
@@ -155,7 +157,8 @@ SC_API size_t sc_qwen2_process_logits_scratch(int64_t rows, int64_t vocab);
 
 /* Logits [rows][vocab] of dtype (SC_F32, SC_F16, SC_BF16), rows `stride` apart, of the tokens vocab_begin ..
  * vocab_begin + vocab (a tensor-parallel rank's slice; every id below is of the whole vocabulary) ->
- * out (out_stride apart; may be logits itself).  Per row and token v, in f32 and rounded once:
+ * out (out_stride apart; may be logits itself with the same stride, or none of its elements).  Per row and
+ * token v, in f32 and rounded once:
  *   x = logits[v]
  *   v among the row's history: x = x > 0 ? x / repetition : x * repetition
  *   x = x - frequency * n - (n > 0 ? presence : 0), n = times v occurs among the generated tokens

@@ -111,6 +111,12 @@ sc_status cuda_fail(cudaError_t e, const char* what);
 // Dynamic shared memory of the router kernels (the token row, f16): K <= 65536.
 constexpr int kRouterMaxRowBytes = 128 * 1024;
 
+// Whether [a, a + a_bytes) and [b, b + b_bytes) share a byte.
+inline bool ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
+
 int sm_count();  // multiprocessors of the current device (148 where there is none)
 
 // Kernels this library has launched (host-side count of launch calls, sc_launch_count).

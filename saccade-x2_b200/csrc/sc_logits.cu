@@ -426,7 +426,16 @@ sc_status sc_qwen2_process_logits(const void* logits, int dtype, int64_t rows, i
     if (mask && (mask_words < (vocab_begin + vocab + 31) / 32 || mask_rows < 0))
         return bad("a mask must cover the vocabulary");
     if (mask && !mask_row && mask_rows < rows) return bad("fewer masks than rows");
-    const uintptr_t size = dtype == SC_F32 ? 4 : 2;
+    const intptr_t size = dtype == SC_F32 ? 4 : 2;
+    if (ranges_meet(logits, ((rows - 1) * stride + vocab) * size, out, ((rows - 1) * out_stride + vocab) * size)) {
+        // in place, or columns of one buffer beside each other
+        const intptr_t apart = reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(logits);
+        intptr_t between = rows > 1 ? apart % (stride * size) : apart;
+        if (between < 0) between += stride * size;
+        if (rows > 1 && stride != out_stride) return bad("out lies over logits with another stride");
+        if (apart != 0 && (rows == 1 || between < vocab * size || between > (stride - vocab) * size))
+            return bad("out lies over logits, but not in place");
+    }
     if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % size)
         return bad("logits and out must be aligned to their type");
     LogitArgs a = {};

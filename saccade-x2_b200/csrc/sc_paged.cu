@@ -377,9 +377,13 @@ sc_status sc_qwen2_paged_append(const void* q, const void* k, const void* v, int
     if (max_pos <= 0) return paged_bad(who, "empty rotation tables");
     const int64_t qw = static_cast<int64_t>(num_heads) * head_dim, kw = static_cast<int64_t>(num_kv_heads) * head_dim;
     if (tokens > 1 && (q_stride < qw || k_stride < kw || v_stride < kw)) return paged_bad(who, "rows overlap");
-    if (q_out == q && (in_dtype != cache_dtype || (tokens > 1 && q_stride != qw)))
-        return paged_bad(who, "in place needs contiguous rows of the cache's type");
     const int64_t is = elem_size(in_dtype), cs = elem_size(cache_dtype);
+    if (q_out == q ? in_dtype != cache_dtype || (tokens > 1 && q_stride != qw)
+                   : ranges_meet(q_out, tokens * qw * cs, q, ((tokens - 1) * q_stride + qw) * is))
+        return paged_bad(who, "in place needs contiguous rows of the cache's type");
+    if (ranges_meet(q_out, tokens * qw * cs, k, ((tokens - 1) * k_stride + kw) * is) ||
+        ranges_meet(q_out, tokens * qw * cs, v, ((tokens - 1) * v_stride + kw) * is))
+        return paged_bad(who, "q_out lies over k or v");
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % is ||
         reinterpret_cast<uintptr_t>(q_out) % cs ||
         (reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) % 4)
@@ -438,7 +442,11 @@ sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* 
     if (max_q_len <= 0 || max_kv_len <= 0) return paged_bad(who, "max_q_len and max_kv_len must be positive");
     if (!(scale > 0.0f) || scale - scale != 0.0f) return paged_bad(who, "scale must be positive and finite");
     const int64_t cs = elem_size(cache_dtype);
-    if (tokens > 1 && q_stride < static_cast<int64_t>(num_heads) * head_dim) return paged_bad(who, "rows of q overlap");
+    const int64_t qw = static_cast<int64_t>(num_heads) * head_dim;
+    if (tokens > 1 && q_stride < qw) return paged_bad(who, "rows of q overlap");
+    if (q == out ? out_dtype != cache_dtype || (tokens > 1 && q_stride != qw)
+                 : ranges_meet(out, tokens * qw * elem_size(out_dtype), q, ((tokens - 1) * q_stride + qw) * cs))
+        return paged_bad(who, "out over q needs contiguous rows of q's type");
     if (!aligned16(q) || (tokens > 1 && q_stride * cs % 16) || !aligned16(k_pages) || !aligned16(v_pages) ||
         page_stride * cs % 16 || !aligned16(out))
         return paged_bad(who, "q, the pages, their strides and out must be 16-byte aligned");
