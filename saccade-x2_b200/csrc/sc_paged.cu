@@ -276,7 +276,7 @@ struct PagedPlan {
 };
 static PagedPlan paged_plan(int dtype, int64_t num_seqs, int nh, int nkv, int hd, int64_t max_q, int64_t max_kv) {
     const int G = nh / nkv, sms = sm_count();
-    const bool few = max_q * G <= 16;
+    const bool few = max_q <= 16 / G;
     PagedPlan p{};
     int64_t share = 0;  // positions of a clustered CTA at most
     if (dtype == SC_F32) {
@@ -329,7 +329,7 @@ static sc_status make_paged(const char* who, const void* k, const void* v, int d
         return paged_bad(who, "page_size must be a power of two in 8..256");
     if (num_pages <= 0 || num_pages > 0x7fffffff || page_stride < static_cast<int64_t>(nkv) * page_size * hd)
         return paged_bad(who, "pages overlap, or none");
-    if (max_pages <= 0 || max_pages * page_size > 0x7fffffff) return paged_bad(who, "max_pages out of range");
+    if (max_pages <= 0 || max_pages > 0x7fffffff / page_size) return paged_bad(who, "max_pages out of range");
     if (num_seqs <= 0 || num_seqs > (1 << 20) || tokens > 0x7fffffff / nh)
         return paged_bad(who, "too many sequences or tokens");
     const uintptr_t size = static_cast<uintptr_t>(elem_size(dtype));
