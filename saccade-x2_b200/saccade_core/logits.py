@@ -12,7 +12,7 @@ from typing import Dict, Optional, Sequence, Union
 
 import torch
 
-from .paged import _serve  # bound to the library there
+from .paged import _serve  # bound to the library there, or missing
 
 MAX_HISTORY = 524287  # ids of a row's history (sc_qwen2_process_logits)
 

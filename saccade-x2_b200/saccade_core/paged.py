@@ -20,7 +20,6 @@ from typing import List, Optional, Set
 
 import torch
 
-from . import _serve
 from ._lib import LIB, SC_EDEVICE, SC_ETIMEOUT, CTarqError, check
 from .op import _DT
 
@@ -31,7 +30,24 @@ def _status_check(status: int) -> None:
 
 _ENTRY_POINTS = ("sc_qwen2_paged_append", "sc_qwen2_paged_attention", "sc_qwen2_paged_attention_scratch",
                  "sc_qwen2_process_logits", "sc_qwen2_process_logits_scratch")
-_serve.bind(_status_check, {n: ctypes.cast(getattr(LIB, n), ctypes.c_void_p).value for n in _ENTRY_POINTS})
+
+
+class _Missing:
+    """In the module's place where it is not built or does not load: the rest of the package works without it."""
+
+    def __init__(self, why: ImportError):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise ImportError(f"saccade_core._serve.{name}: the serving operators' module is missing (make -C csrc builds it)"
+                          ) from self._why
+
+
+try:
+    from . import _serve
+    _serve.bind(_status_check, {n: ctypes.cast(getattr(LIB, n), ctypes.c_void_p).value for n in _ENTRY_POINTS})
+except ImportError as why:
+    _serve = _Missing(why)
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
