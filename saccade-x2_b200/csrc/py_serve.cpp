@@ -154,6 +154,15 @@ int64_t integer(PyObject* o, const char* what) {
     return v;
 }
 
+bool truth(PyObject* o, const char* what) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        throw std::invalid_argument(std::string(what) + " must be true or false");
+    }
+    return v != 0;
+}
+
 // paged_append(q, k, v, cos, sin, k_pages, v_pages, block_table, cu_q, kv_len, out, status)
 PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!takes(n, 12)) return nullptr;
@@ -222,7 +231,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (odt < 0) odt = c.dtype;
         require(odt == c.dtype || (c.dtype == SC_F32 && odt == SC_F16),
                 "out must be of the cache's type, or float16 from a float32 cache");
-        const bool want_lse = PyObject_IsTrue(a[11]) == 1;
+        const bool want_lse = truth(a[11], "return_lse");
         uint32_t* st = status_ptr(a[12], c.dev);
         const On on(c.dev);
         const at::TensorOptions opt = q.options().requires_grad(false);
@@ -323,7 +332,7 @@ PyObject* process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
         } else {
             require(none(a[11]), "mask_row needs a mask");
         }
-        const bool want = PyObject_IsTrue(a[14]) == 1;
+        const bool want = truth(a[14], "return_best");
         uint32_t* st = status_ptr(a[15], dev);
         const On on(dev);
         const at::TensorOptions opt = x.options().requires_grad(false);
