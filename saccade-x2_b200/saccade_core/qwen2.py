@@ -520,7 +520,7 @@ def best_of_ranks(m: Qwen2Model, val: torch.Tensor, idx: torch.Tensor, out: torc
     """The first of the ranks' maxima (val, global idx [n]) into out; cand [n, 2] and gath [world, n, 2] f32 buffers."""
     cand[:, 0].copy_(val)
     cand[:, 1].copy_(idx)  # ids < 2^24 are exact in f32
-    torch.distributed.all_gather_into_tensor(gath, cand, group=m.group)
+    torch.distributed.all_gather_into_tensor(gath.view(-1, 2), cand, group=m.group)
     best = torch.argmax(gath[:, :, 0], dim=0)  # first rank holding the maximum
     out.copy_(gath[:, :, 1].gather(0, best[None, :])[0].to(torch.int64))
     return out
