@@ -140,9 +140,12 @@ SC_API size_t sc_qwen2_paged_attention_scratch(int64_t num_seqs, int num_heads, 
  * bytes.  lse (nullable, f32 [tokens][num_heads]) = log sum exp(scale * q . k).
  * A token at a negative position attends nothing: its output is 0, its lse -inf.  max_q_len and max_kv_len bound
  * every sequence's new tokens and positions and choose the kernels (a sequence with more new tokens is skipped and
- * recorded; more positions are attended all the same).  16-bit caches need q, the pages and their strides 16-byte
- * aligned and run on the tensor cores.  Whatever lies behind a token's position, NaN and infinities too, does not
- * touch its output; one that attends a key that is NaN or a value that is not finite gets no finite result from it. */
+ * recorded; more positions are attended all the same).  q, the pages, their strides and out are 16-byte aligned.
+ * 16-bit caches run on the tensor cores.  With more than 16 rows (max_q_len x query heads of a KV head) each softmax
+ * weight is rounded once to the cache's type there (f16: at worst to steps of 2^-30 of the row's largest), with fewer
+ * it is held in two such parts; the softmax's sums are of the unrounded weights.  Whatever lies behind a token's
+ * position, NaN and infinities too, does not touch its output; one that attends a key that is NaN or a value that is
+ * not finite gets no finite result from it (nor may one of a bf16 cache with values above 2^64). */
 SC_API sc_status sc_qwen2_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                                           int cache_dtype, int64_t num_pages, int64_t page_stride, int page_size,
                                           const int32_t* block_table, int64_t max_pages, const int32_t* cu_q,

@@ -62,3 +62,25 @@ def test_small_weights_of_few_new_tokens_add_up(sc, dtype, heads, lens, bound, s
     err = (out[:end].cpu().double() - ref[:end]).abs()
     assert (ref[:end] > 0).all() and (err <= tol[:end]).all(), float((err / tol[:end]).max())
     assert ((lse[:end].cpu().double() - rl[:end]).abs() <= ltol[:end]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("lens", [[(40, 20011), (3, 900)], [(150, 5000)]], ids=["long", "chunk"])
+@pytest.mark.parametrize("score", [12.0, 20.0])
+def test_small_weights_of_many_new_tokens_add_up(sc, dtype, heads, lens, score):
+    """The plain case's bound without its allowance for weights that f16 cannot hold: the kernel of many new tokens
+    holds a weight in one part, of which the largest is 2^6 at least, so f16's half step of 2^-25 is 2^-31 of it."""
+    c = sink_case(lens, heads, score, dtype, seed=int(score) + len(lens))
+    out = torch.full((c.tokens, c.nh, c.hd), 7.0, dtype=dtype, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    sc.paged_attention(c.q, c.k_pages, c.v_pages, c.table, c.cu_q, c.kv_len, c.max_q, c.max_kv, scale=1.0, out=out,
+                       status=status)
+    torch.cuda.synchronize()
+    assert int(status.item()) == 0 and (out[c.cu[-1]:] == 7.0).all()
+    ref, _, tol, _ = c.attention(1.0)
+    if dtype == torch.float16:
+        tol = tol - _tiny(dtype) + 2.0 ** -25 + 2.0 ** -31 * 1.5 * max(kv for _, kv in lens)
+    end = c.cu[-1]
+    err = (out[:end].cpu().double() - ref[:end]).abs()
+    assert (ref[:end] > 0).all() and (err <= tol[:end]).all(), float((err / tol[:end]).max())
