@@ -96,8 +96,8 @@ class PagedKVCache:
 
     def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, *, max_seqs: int,
                  max_positions: int, dtype: torch.dtype = torch.float16, device="cuda:0"):
-        if layers < 1 or num_pages < 1 or max_seqs < 1 or max_positions < 1:
-            raise ValueError("a cache needs layers, pages, sequences and positions")
+        if layers < 1 or num_pages < 1 or kv_heads < 1 or max_seqs < 1 or max_positions < 1:
+            raise ValueError("a cache needs layers, pages, KV heads, sequences and positions")
         if page_size < 8 or page_size > 256 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two in 8..256")
         if head_dim not in (64, 128):

@@ -820,6 +820,8 @@ class PagedDecoder:
     def generate(self, prompts, steps: int, *, chunk: int = 2048, max_tokens: int = 32768,
                  graph: bool = True) -> torch.Tensor:
         """Tokens [batch, steps] after the prompts."""
+        if steps < 1:
+            raise ValueError("steps must be at least 1")
         out = [self.start(prompts, chunk, max_tokens)]
         if graph and self.graph is None and steps > 1:
             self.capture()
