@@ -2,8 +2,8 @@
 // (saccade_core/paged.py, saccade_core/logits.py) as one CPython call each.
 //
 // A decode step's operators run for 4 to 10 us on the device, less than their argument checks took in
-// Python (24 us a call at first, 15 us when trimmed); here a call's host side is 6 to 8 us, most of it the
-// launches.  The library's entry points come as addresses from the ctypes binding (bind), so
+// Python (24 us a call at first, 15 us when trimmed); here a call's host side is 4 us (append) to 8 us (logits with
+// the best token: two kernels), most of it the launches.  The library's entry points come as addresses from the ctypes binding (bind), so
 // there is one library, whatever SACCADE_CTARQ_LIB says.
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDACachingAllocator.h>

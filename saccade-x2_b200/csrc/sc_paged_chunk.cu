@@ -18,10 +18,10 @@
 // (2^14 in f16): O is then rescaled in tensor memory, which is rare after the first tiles.
 // Pieces of the line of key tiles go to the CTAs evenly (sc_paged.cuh).
 // Measured: 4 x 512 new tokens over 7001..8192 positions, bf16, 64 + 8 heads of 128: 464 us at a full clock (1010
-// TFLOP/s), 520 to 540 under the power cap (990 W at 1.6 GHz; 870); 16 prompts of 129..512 tokens, f16, 28 + 4 heads: 71 us.
+// TFLOP/s), 528 to 556 under the power cap (990 W at 1.6 GHz; 840 to 887); 16 prompts of 129..512 tokens, f16, 28 + 4 heads: 71 us.
 // What bounds it is each half's chain: softmax 1850 cycles, then P V and the next S 1420 with their hand-overs, 3600
 // per pair of tiles where the tensor pipe alone needs 2048 (it is active 51 % of the time, the special-function units
-// 51 %).  Tensor memory is full (S and O of two halves), so S cannot run ahead.  Tried on the first case: 16 softmax
+// 51 %).  Its registers spill (472 bytes stored, 436 loaded at head_dim 128).  Tensor memory is full (S and O of two halves), so S cannot run ahead.  Tried on the first case: 16 softmax
 // warps of 16 rows each 465 us, the same with S ahead in steps of 64 positions (N = 64 products) 570, a tensor-core warp
 // per half and P handed over in two parts 543, the halves' exponentials strictly in turn 521, a quarter of them as
 // polynomials on the FMA pipe 10 to 25 us more each time, row sums in place of maxima to tell when a reference

@@ -1,12 +1,13 @@
 // sc_paged_f32.cu -- attention over an f32 paged cache, in f32 on the CUDA cores.
 //
 // No tensor-core format holds 24 bits, so the products are f32 FMAs, two to an instruction
-// (fma.rn.f32x2).  What bounds them is shared memory: a thread takes 4 rows x (1 or 4) keys of S and 4 rows x
+// (fma.rn.f32x2).  Their operands come from shared memory: a thread takes 4 rows x (1 or 4) keys of S and 4 rows x
 // hd / 16 columns of O, 16-byte loads along head_dim and along the columns.  A row tile has 64 rows, or 16 for few
 // new tokens; there the 16 positions of a quarter of the key tile go to a quarter of the threads
 // with a running maximum and sum of its own, joined at the item's end, so that every thread keeps 4 rows.
 // K and V tiles of 64 positions come by 16-byte asynchronous copies, the next K while O is updated, the
-// next V while S is computed; rows padded by 16 bytes keep 8 of them on different banks.  Positions behind
+// next V while S is computed, with four barriers a tile: the kernel waits more than it issues (31 % of the cycles at 12
+// sequences of 1..24 new tokens); rows padded by 16 bytes keep 8 of them on different banks.  Positions behind
 // the last one are zero-filled.  Pieces of the line of key tiles go to the CTAs evenly (sc_paged.cuh); few new
 // tokens whose CTAs would have at most kClusterKeysF32 positions each go to clusters as in sc_paged_decode.cu (one
 // sequence of 1..256 positions, 28 + 4 heads of 128: 12.2 us cut, 8.4 us in clusters; 4 of 513..1024 16.2 and 18.5;
