@@ -30,8 +30,8 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
       in the row's history:  x = x / repetition where x > 0, x * repetition elsewhere
       n times among its generated tokens:  x = x - frequency * n - (presence if n > 0)
       x = x + the token's (last) bias entry;  -inf where the row's mask does not allow the token
-    history int32 [rows, width <= MAX_HISTORY]: the first hist_len[r] ids are row r's, the first prompt_len[r] of them its
-    prompt (no prompt_len: all generated); ids of other tokens than the slice's are passed over.
+    history int32 [rows, width <= MAX_HISTORY]: the first hist_len[r] ids are row r's, the first prompt_len[r] of
+    them its prompt (no prompt_len: all generated); ids of other tokens than the slice's are passed over.
     repetition (> 0), presence, frequency: f32 [rows].  bias_ids / bias_vals entries bias_ptr[r]..bias_ptr[r + 1]
     (int32 [rows + 1]) are row r's, at most 4095 of them.  mask int32 [masks, words]: bit v % 32 of word
     v / 32 allows token v; mask_row int32 [rows] names each row's mask, negative for none (without it row r has

@@ -58,9 +58,9 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     into the pages and returns the rotated q [tokens, heads, head_dim] in the cache's type.
     q [tokens, heads, head_dim], k and v [tokens, kv heads, head_dim]: f32 or the cache's type, rows any
     distance apart (slices of one projection buffer).  out: where the rotated q goes (q itself works when
-    it is contiguous and of the cache's type; it must not lie over q, k or v otherwise).  Rows behind the last sequence are left as they were, so
-    with out=None their part of the result holds nothing.  status: int32 device word that a position or page
-    outside the tables sets."""
+    it is contiguous and of the cache's type; it must not lie over q, k or v otherwise).  Rows behind the last
+    sequence are left as they were, so with out=None their part of the result holds nothing.  status: int32 device
+    word that a position or page outside the tables sets."""
     return _serve.paged_append(q, k, v, cos, sin, k_pages, v_pages, block_table, cu_q, kv_len, out, status)
 
 
@@ -72,10 +72,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """Causal attention of each sequence's new tokens over its cached positions (the new ones among them):
     out [tokens, heads, head_dim] = softmax(scale * q . k) v, and with return_lse also the f32
     [tokens, heads] log sum exp of the scores.  q [tokens, heads, head_dim] of the cache's type; scale
-    1 / sqrt(head_dim) by default; out_dtype the cache's (or f16 from an f32 cache).  out may be a contiguous q.  max_q_len and
-    max_kv_len bound every sequence's new and cached lengths (they may be larger: a captured graph takes
-    the capacity).  A token at a negative position attends nothing: 0, lse -inf.  Rows behind the last
-    sequence are left as they were."""
+    1 / sqrt(head_dim) by default; out_dtype the cache's (or f16 from an f32 cache).  out may be a contiguous
+    q.  max_q_len and max_kv_len bound every sequence's new and cached lengths (they may be larger: a captured
+    graph takes the capacity).  A token at a negative position attends nothing: 0, lse -inf.  Rows behind the
+    last sequence are left as they were."""
     if out_dtype is None:
         code = -1
     elif out_dtype in _DT:
@@ -137,6 +137,8 @@ class PagedKVCache:
         if positions < 0 or positions > self.max_positions:
             raise ValueError(f"{positions} positions: the cache is made for up to {self.max_positions}")
         have = self._pages[self._slot(slot)]
+        if self.decoder() is None:
+            self._claimed.discard(slot)  # of a decoder that is gone: it is kept, for this caller
         need = -(-positions // self.page_size) - len(have)
         if need <= 0:
             return

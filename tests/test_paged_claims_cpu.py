@@ -83,3 +83,20 @@ def test_a_claimed_slot_that_is_released_by_hand_is_still_given_back():
     c.reserve(1, 20)
     c.give_back(d)
     assert c.free_pages == 10
+
+
+def test_a_dropped_decoders_slot_that_is_reserved_on_is_kept():
+    """The slot is its user's from then on, with the pages that it has, also where pages run short."""
+    c, d = cache(), Decoder()
+    c.claim(d, 3, None)
+    for slot in range(3):
+        c.reserve(slot, 48)
+    before = c.pages(0)
+    del d
+    c.reserve(0, 80)  # two more than its three, of one free: those of the other slots come back
+    assert c.pages(0)[:3] == before and len(set(c.pages(0))) == 5 and c.block_table[0, :5].tolist() == c.pages(0)
+    assert c.free_pages == 5 and c.pages(1) == c.pages(2) == []
+    c.claim(Decoder(), 2, None)
+    assert len(c.pages(0)) == 5
+    c.release(0)
+    assert c.free_pages == 10
